@@ -82,6 +82,11 @@ __device__ __forceinline__ void split_check(float, _Float16, int) {}
 #define HOPMI_SPLIT_STATUS_SETTER(name)
 #endif
 
+// a running statistic's update, (1 - momentum) r + momentum s, with its one fused step spelled out: three kernels apply it (the layer's
+// finalisation, the stack's, the replay for a reused audio branch) and have to agree bit for bit, which an expression left to the
+// compiler's choice of contraction does not give
+__device__ __forceinline__ float running_update(float r, float s, float momentum) { return fmaf(momentum, s, (1.f - momentum) * r); }
+
 __device__ __forceinline__ unsigned wave_max_u32(unsigned m) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, o));

@@ -568,8 +568,8 @@ __global__ __launch_bounds__(256) void wn_bn_finalize_kernel(const float* __rest
     mean_rstd_out[C + c] = rstd;
     mean_rstd_out[2 * C + c] = (float)unbiased;
     if (running_mean != nullptr) {
-      running_mean[c] = (1.f - momentum) * running_mean[c] + momentum * (float)mean;
-      running_var[c] = (1.f - momentum) * running_var[c] + momentum * (float)unbiased;
+      running_mean[c] = running_update(running_mean[c], (float)mean, momentum);
+      running_var[c] = running_update(running_var[c], (float)unbiased, momentum);
     }
   }
 }
@@ -578,8 +578,8 @@ __global__ __launch_bounds__(256) void wn_bn_finalize_kernel(const float* __rest
 __global__ __launch_bounds__(64) void wn_bn_replay_kernel(const float* __restrict__ stats, float* __restrict__ running_mean,
                                                           float* __restrict__ running_var, float momentum) {
   const int c = threadIdx.x;
-  running_mean[c] = (1.f - momentum) * running_mean[c] + momentum * stats[c];
-  running_var[c] = (1.f - momentum) * running_var[c] + momentum * stats[2 * C + c];
+  running_mean[c] = running_update(running_mean[c], stats[c], momentum);
+  running_var[c] = running_update(running_var[c], stats[2 * C + c], momentum);
 }
 
 // forward tiling: one 8-wave workgroup per CU, tiles of up to 80 rows, sized so that the grid covers the launch in one

@@ -768,8 +768,8 @@ __global__ __launch_bounds__(STK_THREADS) void wn_stack_fwd_kernel(StackArgs A) 
           mr[C + tid] = rstd;
           mr[2 * C + tid] = unbiased;
           if (L.rmean != nullptr) {
-            L.rmean[tid] = (1.f - A.momentum) * L.rmean[tid] + A.momentum * (float)mean;
-            L.rvar[tid] = (1.f - A.momentum) * L.rvar[tid] + A.momentum * unbiased;
+            L.rmean[tid] = running_update(L.rmean[tid], (float)mean, A.momentum);
+            L.rvar[tid] = running_update(L.rvar[tid], (float)unbiased, A.momentum);
           }
         }
       }
