@@ -11,6 +11,7 @@ _lib = None
 
 _F = ctypes.POINTER(ctypes.c_float)
 _I = ctypes.c_int
+_LL = ctypes.c_longlong
 _VP = ctypes.c_void_p
 
 # name -> (restype, argtypes); must list every symbol include/hopmi.h declares
@@ -109,6 +110,17 @@ SIGNATURES = {
     "hopmi_gru_bwd_operands": (_I, [_VP, _VP, _VP, _VP, _I, _I, _I, _VP]),
     "hopmi_gru_bwd_ws_floats": (ctypes.c_size_t, [_I, _I]),
     "hopmi_gru_bwd": (_I, [_VP] * 8 + [_I, _I, _I, _VP]),
+    "hopmi_layernorm_fwd": (_I, [_VP, _LL, _VP, _VP, _I, _VP, _VP, _VP, _I, _I, ctypes.c_float, _I, _VP]),
+    "hopmi_layernorm_bwd_ws_floats": (ctypes.c_size_t, [_I, _I, _I]),
+    "hopmi_layernorm_bwd": (_I, [_VP, _LL, _VP, _VP, _VP, _VP, _I, _VP, _VP, _VP, _VP, _I, _I, _I, _VP]),
+    "hopmi_gemm16_ws_floats": (ctypes.c_size_t, [_I, _I, _I, _I]),
+    "hopmi_gemm16_direct": (_I, [_VP, _LL, _I]),
+    "hopmi_gemm16": (_I, [_VP, _LL, _VP, _LL, _I, _VP, _LL, _VP, _VP, _LL, _VP, _LL, _I, _I, _I, _I, _I, _VP, _VP]),
+    "hopmi_pad16": (_I, [_VP, _LL, _VP, _LL, _I, _I, _VP]),
+    "hopmi_act_bwd16_ws_floats": (ctypes.c_size_t, [_I, _I]),
+    "hopmi_act_bwd16": (_I, [_VP, _LL, _VP, _LL, _VP, _LL, _VP, _VP, _I, _I, _I, _I, _VP]),
+    "hopmi_grad_clip_ws_bytes": (ctypes.c_size_t, []),
+    "hopmi_grad_clip": (_I, [_VP, _VP, _VP, _VP, _I, ctypes.c_float, _VP, _VP, _VP]),
     "hopmi_adam_chunk": (_I, []),
     "hopmi_adam_multi": (_I, [_VP, _VP, _I, ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double, _VP, _VP]),
 }

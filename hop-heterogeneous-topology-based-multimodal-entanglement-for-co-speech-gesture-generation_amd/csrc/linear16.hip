@@ -1,0 +1,617 @@
+// Matrix products of 16-bit operands (bf16 or fp16, fp32 accumulation) with bias, activation and residual in the epilogue, and the
+// products of their backward pass:
+//
+//   forward    z = X W^T + b,  Y = act(z) + R              X [M][K], W [N][K]: both contiguous along the contraction
+//   backward   dz = dY act'(z),  db = sum_rows dz          (one element-wise pass; dz rounded once, to the operands' type)
+//              dX = dz W                                   W [N][K] contiguous along the RESULT's columns
+//              dW = dz^T X                                 both contiguous along the result's sides, contraction over the rows
+//
+// One kernel covers the three: each operand's tile is staged into LDS by LDS-DMA (global_load_lds, 16 bytes per lane, no registers in
+// between) in the order in which it lies in memory, and read as MFMA fragments either straight (contraction-contiguous: ds_read_b128)
+// or through the transposing LDS read (ds_read_b64_tr_b16), so no operand is ever transposed in memory.
+// v_mfma_f32_16x16x32: lane 16 q + n holds A[n][8 q ..], B[8 q ..][n] and D[4 q + r][n].  The result's COLUMNS are put on D's rows, so a
+// lane ends with four consecutive columns of one row and every epilogue access is 8 bytes.
+// LDS images are swizzled through the SOURCE address of each lane's 16 bytes (the DMA's LDS side is fixed: lane l at base + 16 l):
+//   contraction-contiguous tile [rows][64]: 128-byte rows, chunk c at c ^ ((row >> 1) & 7): 16 consecutive rows on 16 different slots
+//   result-contiguous tile [64][cols]: row k, 32-byte pair p at p ^ ((k & 3) | ((k >> 3) & 1) << 2): the eight rows that one half wave
+//   reads lie on eight different 32-byte groups
+// Edges: rows past the end are clamped to the last one (their results are not stored); contraction indices past the end read 16 bytes
+// of zeros instead, on both operands.  Operands whose rows do not start on 16 bytes, or end inside one, are copied once into rows
+// padded with zeros.
+#include "t16_dev.h"
+
+namespace hopmi {
+
+enum { ACT_NONE = 0, ACT_RELU = 1, ACT_GELU = 2, ACT_SILU = 3 };
+
+__device__ __attribute__((aligned(16))) const unsigned g_zero16[4] = {0, 0, 0, 0};
+
+typedef __bf16 bfrag __attribute__((ext_vector_type(8)));
+typedef _Float16 hfrag __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ f32x4 mfma16x32(u32x4_t a, u32x4_t b, f32x4 c, const __bf16*) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bfrag, a), __builtin_bit_cast(bfrag, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma16x32(u32x4_t a, u32x4_t b, f32x4 c, const _Float16*) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(hfrag, a), __builtin_bit_cast(hfrag, b), c, 0, 0, 0);
+}
+
+// The normal distribution's tail, Phi(-u) for u >= 0, = exp(-u^2 / 2) Q(t) with t = 1 / (1 + p u): Q is e^{x^2} erfc(x) / 2 at x = u / sqrt 2,
+// a smooth function that a polynomial in t without constant term (Q -> 0 with t) meets to 5e-6 of its value on 0 <= u <= 14 (least
+// largest relative error, fitted against 64-bit values); beyond, exp(-u^2 / 2) is 0 in fp32.  RELATIVE accuracy far below the result's
+// rounding (2^-9 / 2^-12) also in the tail, at 11 instructions (erff takes several times that, in an epilogue that runs against MFMAs).
+__device__ __forceinline__ float gauss_tail(float u, float e) {      // e = exp(-u^2 / 2)
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.31f, u, 1.f));
+  float q = fmaf(-0.07392919063568115f, t, 0.18044988811016083f);
+  q = fmaf(q, t, 0.01574617065489292f);
+  q = fmaf(q, t, 0.13342832028865814f);
+  q = fmaf(q, t, 0.12044187635183334f);
+  q = fmaf(q, t, 0.12386061996221542f);
+  return q * t * e;
+}
+// silu is taken from h = exp(-|z| / 2): z h h keeps the negative tail where exp(z) itself would have left fp32's normal range.
+// Where a tail has underflowed the limits (z or 0) stand, at the infinities too; a NaN stays one.
+__device__ __forceinline__ float act_fwd(float z, int act) {
+  if (act == ACT_RELU) return z > 0.f || z != z ? z : 0.f;
+  if (act == ACT_GELU) {
+    const float tail = gauss_tail(fabsf(z), __expf(-0.5f * z * z));
+    return tail > 0.f || z != z ? (z > 0.f ? fmaf(-z, tail, z) : z * tail) : (z > 0.f ? z : -0.f);
+  }
+  if (act == ACT_SILU) {
+    const float h = __expf(-0.5f * fabsf(z)), d = __builtin_amdgcn_rcpf(fmaf(h, h, 1.f));
+    return z > 0.f ? z * d : (h > 0.f ? z * h * h * d : (z != z ? z : -0.f));
+  }
+  return z;
+}
+__device__ __forceinline__ float act_grad(float z, int act) {
+  if (act == ACT_RELU) return z > 0.f ? 1.f : 0.f;
+  if (act == ACT_GELU) {
+    const float e = __expf(-0.5f * z * z), tail = gauss_tail(fabsf(z), e);
+    return fmaf(e > 0.f || z != z ? z * 0.3989422804014327f : 0.f, e, z > 0.f ? 1.f - tail : tail);
+  }
+  if (act == ACT_SILU) {
+    const float h = __expf(-0.5f * fabsf(z)), e = h * h, d = __builtin_amdgcn_rcpf(1.f + e);
+    const float s = z > 0.f ? d : e * d, r = z > 0.f ? e * d : d;      // the sigmoid and what it lacks to 1
+    return e > 0.f || z != z ? s * fmaf(z, r, 1.f) : (z > 0.f ? 1.f : 0.f);
+  }
+  return 1.f;
+}
+
+// four consecutive elements at any element address
+template <typename T> __device__ __forceinline__ void ld4f(const T* p, float (&f)[4]) {
+  const u32x2_any v = *reinterpret_cast<const u32x2_any*>(p);
+  const u32x4_t w = {v[0], v[1], 0, 0};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) f[e] = vget(w, e, p);
+}
+template <typename T> __device__ __forceinline__ void st4f(T* p, const float (&f)[4]) {
+  u32x2_any v;
+  v[0] = pk2(f[0], f[1], p);
+  v[1] = pk2(f[2], f[3], p);
+  *reinterpret_cast<u32x2_any*>(p) = v;
+}
+
+template <typename T> struct Epi16 {
+  T* C; long long ldc;
+  const T* bias;                 // [N] or null
+  const T* res; long long ldr;   // [M][N] or null
+  T* z; long long ldz;           // pre-activation values for the backward pass, or null (rounded to the operands' type: what dY act'(z)
+                                 // loses by it is a third of what the rounding of dz itself loses)
+  int act;
+};
+// columns col .. col + 3 of a row, of which `left` (>= 1) exist
+template <typename T> __device__ __forceinline__ void epilogue4(const Epi16<T>& E, long long row, int col, int left, float (&f)[4]) {
+  float t[4];
+  if (left >= 4) {
+    if (E.bias != nullptr) {
+      ld4f(E.bias + col, t);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[e] += t[e];
+    }
+    if (E.z != nullptr) st4f(E.z + row * E.ldz + col, f);
+    if (E.act != ACT_NONE) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[e] = act_fwd(f[e], E.act);
+    }
+    if (E.res != nullptr) {
+      ld4f(E.res + row * E.ldr + col, t);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[e] += t[e];
+    }
+    st4f(E.C + row * E.ldc + col, f);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < left) {
+        float v = f[e];
+        if (E.bias != nullptr) v += to_f(E.bias[col + e]);
+        if (E.z != nullptr) E.z[row * E.ldz + col + e] = (T)v;
+        v = act_fwd(v, E.act);
+        if (E.res != nullptr) v += to_f(E.res[row * E.ldr + col + e]);
+        E.C[row * E.ldc + col + e] = (T)v;
+      }
+  }
+}
+
+template <typename T> struct Gemm16 {
+  const T* A; long long lda;     // the result's rows:    [M][K] (KA) or [K][M]
+  const T* B; long long ldb;     // the result's columns: [N][K] (KB) or [K][N]
+  int M, N, K;
+  Epi16<T> E;
+  float* part;                   // contraction split over several workgroups: fp32 partial results [splits][M][N], else null
+  int tiles_m, tiles_n, splits;
+};
+
+constexpr int G16_BK = 64;       // contraction per step
+
+// Staging of one operand's tile of R rows (KC: [R][64], else [64][R]) by NW waves, and its fragments.
+template <typename T, int R, int NW, bool KC> struct Tile16 {
+  static constexpr int NI = R / 8 / NW;            // 1 KiB DMA instructions per wave and step
+  static constexpr int LPR = KC ? 8 : R / 8;       // lanes per tile row in memory order
+  const char* base;                                // uniform; advances by one step
+  long long adv;
+  unsigned off[NI];                                // this lane's bytes from base
+  int kk[NI];                                      // contraction index (within a step) of this lane's first element
+
+  __device__ __forceinline__ void init(const T* p, long long ld, int r0, int r_total, int k0, int lane, int wave) {
+    if (KC) {
+      base = reinterpret_cast<const char*>(p + (long long)r0 * ld + k0);
+      adv = G16_BK * 2;
+    } else {
+      base = reinterpret_cast<const char*>(p + (long long)k0 * ld + r0);
+      adv = G16_BK * 2 * ld;
+    }
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      if (KC) {
+        const int row = (i * NW + wave) * 8 + (lane >> 3), c = (lane & 7) ^ ((row >> 1) & 7);
+        const int rc = min(row, r_total - 1 - r0);             // (r_total > r0)
+        off[i] = (unsigned)(rc * ld * 2 + c * 16);
+        kk[i] = c * 8;
+      } else {
+        const int k = (i * NW + wave) * (64 / LPR) + lane / LPR, s = lane % LPR;
+        const int c = ((((s >> 1) ^ ((k & 3) | ((k >> 3) & 1) << 2)) << 1) | (s & 1)) * 8;
+        const int cc = min(c, ((r_total - r0 + 7) & ~7) - 8);  // (whole chunks: the operand's rows are padded to 8)
+        off[i] = (unsigned)(k * ld * 2 + cc * 2);
+        kk[i] = k;
+      }
+    }
+  }
+  // issues the step's DMA into `lds`; `left`: contraction indices that exist from this step's start on (KC: rounded up to 8)
+  __device__ __forceinline__ void load(char* lds, int left, int wave) {
+    if (left >= G16_BK) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(base + off[i]),
+                                         (__attribute__((address_space(3))) void*)(lds + (i * NW + wave) * 1024), 16, 0, 0);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const char* src = kk[i] < left ? base + off[i] : reinterpret_cast<const char*>(g_zero16);
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
+                                         (__attribute__((address_space(3))) void*)(lds + (i * NW + wave) * 1024), 16, 0, 0);
+      }
+    }
+    base += adv;
+  }
+};
+
+// fragments of NB 16-row blocks starting at block `b0` of a staged tile, contraction half ks
+template <typename T, int R, int NB, bool KC>
+__device__ __forceinline__ void frags16(const char* lds, int b0, int ks, int n, int q, u32x4_t (&f)[NB]) {
+  if (KC) {
+    const char* p = lds + b0 * 2048 + n * 128 + (((ks * 4 + q) ^ (n >> 1)) << 4);
+#pragma unroll
+    for (int j = 0; j < NB; ++j) f[j] = *reinterpret_cast<const u32x4_t*>(p + j * 2048);
+  } else {
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s4* s4p;
+    const int sw = (n >> 2) | (q & 1) << 2;
+    const char* p = lds + (ks * 32 + 8 * q + (n >> 2)) * (R * 2) + (n & 3) * 8;
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      const char* a = p + (((b0 + j) ^ sw) << 5);
+      const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s4p)(a)), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s4p)(a + 4 * R * 2));
+      typedef unsigned u2 __attribute__((ext_vector_type(2)));
+      const u2 l = __builtin_bit_cast(u2, lo), h = __builtin_bit_cast(u2, hi);
+      f[j] = u32x4_t{l[0], l[1], h[0], h[1]};
+    }
+  }
+}
+
+template <typename T, int BM, int BN, int WR, int WC, bool KA, bool KB>
+__global__ __launch_bounds__(64 * WR * WC) void gemm16_kernel(Gemm16<T> G) {
+  constexpr int NW = WR * WC, RB = BM / WR / 16, CB = BN / WC / 16;
+  constexpr int SA = BM * G16_BK * 2, SB = BN * G16_BK * 2, ST = SA + SB;
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, q = lane >> 4;
+  const int wr = wave / WC, wc = wave % WC;
+  // workgroups go to the eight XCDs in turn: give each XCD one contiguous stretch of the tile order, and walk that order in groups of
+  // eight tile rows, so that what an L2 holds is used by its own workgroups
+  const int tiles = G.tiles_m * G.tiles_n, total = tiles * G.splits;
+  int id = blockIdx.x;
+  {
+    const int per = total / 8, rem = total % 8, x = id % 8, i = id / 8;
+    id = x * per + min(x, rem) + i;
+  }
+  const int split = id / tiles;
+  id -= split * tiles;
+  const int per_group = 8 * G.tiles_n, g = id / per_group, first = g * 8, size = min(8, G.tiles_m - first);
+  const int tm = first + (id - g * per_group) % size, tn = (id - g * per_group) / size;
+  const int r0 = tm * BM, c0 = tn * BN;
+  const int steps = (G.K + G16_BK - 1) / G16_BK;
+  const int s0 = (int)((long long)steps * split / G.splits), s1 = (int)((long long)steps * (split + 1) / G.splits);
+  Tile16<T, BM, NW, KA> ta;
+  Tile16<T, BN, NW, KB> tb;
+  ta.init(G.A, G.lda, r0, G.M, s0 * G16_BK, lane, wave);
+  tb.init(G.B, G.ldb, c0, G.N, s0 * G16_BK, lane, wave);
+  const int ka = KA ? (G.K + 7) & ~7 : G.K, kb = KB ? (G.K + 7) & ~7 : G.K;
+  f32x4 acc[RB][CB];
+#pragma unroll
+  for (int i = 0; i < RB; ++i)
+#pragma unroll
+    for (int j = 0; j < CB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (s0 < s1) {
+    ta.load(lds, ka - s0 * G16_BK, wave);
+    tb.load(lds + SA, kb - s0 * G16_BK, wave);
+  }
+  for (int s = s0; s < s1; ++s) {
+    char* cur = lds + ((s - s0) & 1) * ST;
+    // this step's tiles are in LDS once every wave's DMA is (vmcnt, then the barrier), and every wave is done with the other buffer
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    if (s + 1 < s1) {
+      char* nxt = lds + ((s + 1 - s0) & 1) * ST;
+      ta.load(nxt, ka - (s + 1) * G16_BK, wave);
+      tb.load(nxt + SA, kb - (s + 1) * G16_BK, wave);
+    }
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      u32x4_t fa[RB], fb[CB];
+      frags16<T, BM, RB, KA>(cur, wr * RB, ks, n, q, fa);
+      frags16<T, BN, CB, KB>(cur + SA, wc * CB, ks, n, q, fb);
+#pragma unroll
+      for (int i = 0; i < RB; ++i)
+#pragma unroll
+        for (int j = 0; j < CB; ++j) acc[i][j] = mfma16x32(fb[j], fa[i], acc[i][j], G.A);
+    }
+  }
+  const int row0 = r0 + wr * RB * 16 + n, col0 = c0 + wc * CB * 16 + 4 * q;
+#pragma unroll
+  for (int i = 0; i < RB; ++i) {
+    const long long row = row0 + i * 16;
+    if (row >= G.M) continue;
+#pragma unroll
+    for (int j = 0; j < CB; ++j) {
+      const int col = col0 + j * 16, left = G.N - col;
+      if (left <= 0) continue;
+      float f[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+      if (G.part != nullptr) {
+        float* p = G.part + ((long long)split * G.M + row) * G.N + col;
+        if (left >= 4) *reinterpret_cast<u32x4_any*>(p) = vpack(f, p);
+        else
+          for (int e = 0; e < left; ++e) p[e] = f[e];
+      } else {
+        epilogue4(G.E, row, col, left, f);
+      }
+    }
+  }
+}
+
+// the partial results of a split contraction, added in split order, through the same epilogue; four columns per thread
+template <typename T>
+__global__ __launch_bounds__(256) void gemm16_join_kernel(const float* __restrict__ part, int splits, int M, int N, Epi16<T> E) {
+  const int q4 = (N + 3) / 4;
+  const long long total = (long long)M * q4, plane = (long long)M * N;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+    const long long row = i / q4;
+    const int col = (int)(i - row * q4) * 4, left = N - col;
+    const float* p = part + row * N + col;
+    float f[4] = {0.f, 0.f, 0.f, 0.f};
+    if (left >= 4) {
+#pragma unroll 4
+      for (int s = 0; s < splits; ++s) {
+        const u32x4_t v = ld16(p + s * plane);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[e] += __uint_as_float(v[e]);
+      }
+    } else {
+      for (int s = 0; s < splits; ++s)
+        for (int e = 0; e < left; ++e) f[e] += p[s * plane + e];
+    }
+    epilogue4(E, row, col, left, f);
+  }
+}
+
+// Few rows (M <= 64): bound by reading W once.  A workgroup takes 16 columns of the result for all rows; its eight waves share the
+// contraction in stretches of 128 (256 contiguous bytes of each of 16 rows of W per wave and stretch), straight from memory into MFMA
+// operands at any alignment, and add their partial tiles through LDS.
+constexpr int FEW_ROWS = 64, FEW_WAVES = 8;
+template <typename T, int MB>
+__global__ __launch_bounds__(64 * FEW_WAVES) void gemm16_few_kernel(Gemm16<T> G) {
+  __shared__ float red[FEW_WAVES][MB][16][17];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, q = lane >> 4;
+  const int c0 = blockIdx.x * 16;
+  const T* wp = G.B + (long long)min(c0 + n, G.N - 1) * G.ldb + 8 * q;
+  const T* xp[MB];
+#pragma unroll
+  for (int m = 0; m < MB; ++m) xp[m] = G.A + (long long)min(m * 16 + n, G.M - 1) * G.lda + 8 * q;
+  f32x4 acc[MB];
+#pragma unroll
+  for (int m = 0; m < MB; ++m) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // eight elements from contraction index k on, zeros past the end
+  auto tail8 = [&](const T* p, int k) {
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = k + e < G.K ? to_f(p[e]) : 0.f;
+    return vpack(f, p);
+  };
+  for (int k0 = wave * 128; k0 < G.K; k0 += FEW_WAVES * 128) {
+    if (k0 + 128 <= G.K) {
+      u32x4_t w[4], x[MB][4];
+#pragma unroll
+      for (int s = 0; s < 4; ++s) w[s] = ld16(wp + k0 + 32 * s);
+#pragma unroll
+      for (int m = 0; m < MB; ++m)
+#pragma unroll
+        for (int s = 0; s < 4; ++s) x[m][s] = ld16(xp[m] + k0 + 32 * s);
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int m = 0; m < MB; ++m) acc[m] = mfma16x32(w[s], x[m][s], acc[m], G.A);
+    } else {
+      for (int k = k0; k < G.K; k += 32) {
+        const int kl = k + 8 * q;
+        const u32x4_t w = kl + 8 <= G.K ? ld16(wp + k) : tail8(wp + k, kl);
+#pragma unroll
+        for (int m = 0; m < MB; ++m) {
+          const u32x4_t x = kl + 8 <= G.K ? ld16(xp[m] + k) : tail8(xp[m] + k, kl);
+          acc[m] = mfma16x32(w, x, acc[m], G.A);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < MB; ++m)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) red[wave][m][n][4 * q + r] = acc[m][r];
+  __syncthreads();
+  for (int i = threadIdx.x; i < MB * 64; i += 64 * FEW_WAVES) {
+    const int row = i >> 2, c = (i & 3) * 4, left = G.N - c0 - c;
+    if (row >= G.M || left <= 0) continue;
+    float f[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < FEW_WAVES; ++w)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[e] += red[w][row >> 4][row & 15][c + e];
+    epilogue4(G.E, row, c0 + c, left, f);
+  }
+}
+
+// dz = dY act'(z) (rows padded with zeros to ldd, a multiple of 8; null: not wanted) and the partial column sums of the UNROUNDED dz of
+// each row group, part [gridDim.y][N] (null: not wanted).  A wave takes 512 columns of every fourth row of its group.
+template <typename T>
+__global__ __launch_bounds__(256) void act_bwd16_kernel(const T* __restrict__ dy, long long ldy, const T* __restrict__ z, long long ldz,
+                                                        T* __restrict__ dz, long long ldd, float* __restrict__ part, int M, int N, int act) {
+  __shared__ float red[3][512];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = blockIdx.x * 512 + lane * 8, left = N - col;
+  float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (left > 0)
+    for (long long row = (long long)blockIdx.y * 4 + wave; row < M; row += (long long)gridDim.y * 4) {
+      float g[8], v[8];
+      const T* p = dy + row * ldy + col;
+      if (left >= 8) ldf<8>(p, g);
+      else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) g[e] = e < left ? to_f(p[e]) : 0.f;
+      }
+      if (act != ACT_NONE) {
+        ldf<8>(z + row * ldz + col, v);              // (rows of z are padded to 8)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) g[e] = e < left ? g[e] * act_grad(v[e], act) : 0.f;
+      }
+      if (dz != nullptr) st16(dz + row * ldd + col, vpack(g, p));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[e] += g[e];
+    }
+  if (part == nullptr) return;
+  if (wave > 0) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) red[wave - 1][lane * 8 + e] = s[e];
+  }
+  __syncthreads();
+  if (wave == 0 && left > 0) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < left) part[(long long)blockIdx.y * N + col + e] = s[e] + red[0][lane * 8 + e] + red[1][lane * 8 + e] + red[2][lane * 8 + e];
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(1024) void colsum16_join_kernel(const float* __restrict__ part, int G, int N, T* __restrict__ out) {
+  __shared__ float red[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
+  float s = 0.f;
+  if (c < N)
+#pragma unroll 4
+    for (int g = wave; g < G; g += 16) s += part[(long long)g * N + c];
+  red[wave][lane] = s;
+  __syncthreads();
+  if (wave == 0 && c < N) {
+    float t = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) t += red[k][lane];
+    out[c] = (T)t;
+  }
+}
+
+// rows of N 16-bit elements at any stride and alignment -> rows of ldp (a multiple of 8) elements, zeros behind the N-th (bits are moved,
+// whatever they stand for)
+__global__ __launch_bounds__(256) void pad16_kernel(const unsigned short* __restrict__ src, long long lds_, unsigned short* __restrict__ dst,
+                                                    long long ldp, int M, int N) {
+  const int vecs = (int)(ldp / 8);
+  const long long total = (long long)M * vecs;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+    const long long row = i / vecs;
+    const int col = (int)(i - row * vecs) * 8;
+    const unsigned short* p = src + row * lds_ + col;
+    u32x4_t v = {0, 0, 0, 0};
+    if (col + 8 <= N) v = ld16(p);
+    else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (col + e < N) v[e >> 1] |= (unsigned)p[e] << (16 * (e & 1));
+    }
+    st16(dst + row * ldp + col, v);
+  }
+}
+
+// ---- geometry
+struct Plan16 { int bm, tiles_m, tiles_n, splits; };
+static Plan16 plan16(int M, int N, int K) {
+  Plan16 p;
+  const int steps = (K + G16_BK - 1) / G16_BK;
+  const long long big = (long long)((M + 255) / 256) * ((N + 255) / 256);
+  p.bm = big >= 224 ? 256 : 128;
+  p.tiles_m = (M + p.bm - 1) / p.bm;
+  p.tiles_n = (N + p.bm - 1) / p.bm;
+  const long long tiles = (long long)p.tiles_m * p.tiles_n;
+  p.splits = 1;
+  if (p.bm == 128 && tiles < 256) {
+    const long long want = 512 / tiles, most = steps / 4 > 0 ? steps / 4 : 1;
+    p.splits = (int)(want < most ? want : most);
+    if (p.splits < 1) p.splits = 1;
+  }
+  return p;
+}
+
+template <typename T, int BM, bool KA, bool KB> static void gemm16_go(const Gemm16<T>& G, hipStream_t st) {
+  constexpr int W = BM == 256 ? 8 : 4;
+  constexpr int bytes = 2 * 2 * BM * G16_BK * 2;
+  const unsigned grid = (unsigned)(G.tiles_m * G.tiles_n * G.splits);
+  if constexpr (BM == 256) {
+    static const hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void*>(gemm16_kernel<T, 256, 256, 2, 4, KA, KB>),
+                                                       hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    (void)once;
+    hipLaunchKernelGGL((gemm16_kernel<T, 256, 256, 2, 4, KA, KB>), dim3(grid), dim3(64 * W), bytes, st, G);
+  } else {
+    hipLaunchKernelGGL((gemm16_kernel<T, 128, 128, 2, 2, KA, KB>), dim3(grid), dim3(64 * W), bytes, st, G);
+  }
+}
+template <typename T> static void gemm16_run(Gemm16<T> G, int layout, float* ws, hipStream_t st) {
+  if (layout == 0 && G.M <= FEW_ROWS) {
+    const dim3 grid((G.N + 15) / 16), block(64 * FEW_WAVES);
+    if (G.M <= 16) hipLaunchKernelGGL((gemm16_few_kernel<T, 1>), grid, block, 0, st, G);
+    else if (G.M <= 32) hipLaunchKernelGGL((gemm16_few_kernel<T, 2>), grid, block, 0, st, G);
+    else hipLaunchKernelGGL((gemm16_few_kernel<T, 4>), grid, block, 0, st, G);
+    return;
+  }
+  const Plan16 p = plan16(G.M, G.N, G.K);
+  G.tiles_m = p.tiles_m;
+  G.tiles_n = p.tiles_n;
+  G.splits = p.splits;
+  G.part = p.splits > 1 ? ws : nullptr;
+  if (p.bm == 256) {
+    if (layout == 0) gemm16_go<T, 256, true, true>(G, st);
+    else if (layout == 1) gemm16_go<T, 256, true, false>(G, st);
+    else gemm16_go<T, 256, false, false>(G, st);
+  } else {
+    if (layout == 0) gemm16_go<T, 128, true, true>(G, st);
+    else if (layout == 1) gemm16_go<T, 128, true, false>(G, st);
+    else gemm16_go<T, 128, false, false>(G, st);
+  }
+  if (p.splits > 1) {
+    const long long work = (long long)G.M * ((G.N + 3) / 4), blocks = (work + 255) / 256;
+    hipLaunchKernelGGL((gemm16_join_kernel<T>), dim3((unsigned)(blocks < 2048 ? blocks : 2048)), dim3(256), 0, st, ws, p.splits, G.M, G.N, G.E);
+  }
+}
+
+static bool g16_direct(const void* p, long long ld, int cols) {
+  return !((reinterpret_cast<uintptr_t>(p) & 15) | (ld & 7) | (cols & 7));
+}
+static int act_bwd_groups(int M, int N) {
+  const int strips = (N + 511) / 512;
+  const long long quads = ((long long)M + 3) / 4;
+  long long g = 1024 / strips;
+  g = g < 1 ? 1 : g;
+  return (int)(quads < g ? quads : g);
+}
+
+}  // namespace hopmi
+
+using namespace hopmi;
+
+extern "C" size_t hopmi_gemm16_ws_floats(int M, int N, int K, int layout) {
+  if (M < 1 || N < 1 || K < 1 || layout < 0 || layout > 2) return 0;
+  if (layout == 0 && M <= FEW_ROWS) return 0;
+  const Plan16 p = plan16(M, N, K);
+  return p.splits > 1 ? (size_t)p.splits * M * N : 0;
+}
+
+extern "C" int hopmi_gemm16_direct(const void* p, long long ld, int cols) { return g16_direct(p, ld, cols) ? 1 : 0; }
+
+extern "C" int hopmi_gemm16(const void* A, long long lda, const void* B, long long ldb, int layout, void* C, long long ldc, const void* bias,
+                            const void* res, long long ldr, void* z, long long ldz, int act, int M, int N, int K, int dtype, float* ws,
+                            void* stream) {
+  if (!A || !B || !C) { set_error("hopmi_gemm16: null pointer argument"); return HOPMI_EINVAL; }
+  if (M < 1 || N < 1 || K < 1 || layout < 0 || layout > 2 || act < ACT_NONE || act > ACT_SILU) {
+    set_error("hopmi_gemm16: M=%d N=%d K=%d layout=%d activation=%d", M, N, K, layout, act);
+    return HOPMI_EINVAL;
+  }
+  if (dtype != T_BF16 && dtype != T_F16) { set_error("hopmi_gemm16: dtype=%d (1 bf16, 2 fp16)", dtype); return HOPMI_EINVAL; }
+  const int ca = layout == 2 ? M : K, cb = layout == 0 ? K : N;
+  if (lda < ca || ldb < cb || ldc < N || (res && ldr < N) || (z && ldz < N)) { set_error("hopmi_gemm16: a row stride below the row's length"); return HOPMI_EINVAL; }
+  if (lda > (1 << 22) || ldb > (1 << 22)) { set_error("hopmi_gemm16: row stride above 2^22 elements"); return HOPMI_EINVAL; }
+  const bool few = layout == 0 && M <= FEW_ROWS;
+  if (!few && (!g16_direct(A, lda, 0) || !g16_direct(B, ldb, 0) || lda < ((ca + 7) & ~7) || ldb < ((cb + 7) & ~7))) {
+    set_error("hopmi_gemm16: operands need rows on 16 bytes that end on 16 bytes (hopmi_pad16)");
+    return HOPMI_EINVAL;
+  }
+  if (!few && hopmi_gemm16_ws_floats(M, N, K, layout) > 0 && !ws) { set_error("hopmi_gemm16: null workspace"); return HOPMI_EINVAL; }
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  auto go = [&](auto t) {
+    using T = decltype(t);
+    Gemm16<T> G;
+    G.A = static_cast<const T*>(A); G.lda = lda;
+    G.B = static_cast<const T*>(B); G.ldb = ldb;
+    G.M = M; G.N = N; G.K = K;
+    G.E = Epi16<T>{static_cast<T*>(C), ldc, static_cast<const T*>(bias), static_cast<const T*>(res), ldr, static_cast<T*>(z), ldz, act};
+    G.part = nullptr; G.tiles_m = G.tiles_n = G.splits = 1;
+    gemm16_run(G, layout, ws, st);
+  };
+  if (dtype == T_BF16) go(__bf16{}); else go(_Float16{});
+  return check_launch("hopmi_gemm16");
+}
+
+extern "C" int hopmi_pad16(const void* src, long long lds_, void* dst, long long ldp, int M, int N, void* stream) {
+  if (!src || !dst || M < 1 || N < 1 || lds_ < N || ldp < N || (ldp & 7) || (reinterpret_cast<uintptr_t>(dst) & 15)) {
+    set_error("hopmi_pad16: M=%d N=%d strides %lld -> %lld, or a null or unaligned pointer", M, N, lds_, ldp);
+    return HOPMI_EINVAL;
+  }
+  const long long work = (long long)M * (ldp / 8), blocks = (work + 255) / 256;
+  hipLaunchKernelGGL(pad16_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, static_cast<hipStream_t>(stream),
+                     static_cast<const unsigned short*>(src), lds_, static_cast<unsigned short*>(dst), ldp, M, N);
+  return check_launch("hopmi_pad16");
+}
+
+extern "C" size_t hopmi_act_bwd16_ws_floats(int M, int N) { return M < 1 || N < 1 ? 0 : (size_t)act_bwd_groups(M, N) * N; }
+
+extern "C" int hopmi_act_bwd16(const void* dy, long long ldy, const void* z, long long ldz, void* dz, long long ldd, void* dbias, float* ws,
+                               int act, int M, int N, int dtype, void* stream) {
+  if (!dy || M < 1 || N < 1 || ldy < N || act < ACT_NONE || act > ACT_SILU || (dtype != T_BF16 && dtype != T_F16) || (act != ACT_NONE && !z) ||
+      (z && ldz < ((N + 7) & ~7)) || (dz && (ldd < N || (ldd & 7))) || (dbias && !ws)) {
+    set_error("hopmi_act_bwd16: M=%d N=%d activation=%d dtype=%d, a bad stride, or a null pointer", M, N, act, dtype);
+    return HOPMI_EINVAL;
+  }
+  if (!dz && !dbias) return HOPMI_OK;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const int groups = act_bwd_groups(M, N);
+  auto go = [&](auto t) {
+    using T = decltype(t);
+    hipLaunchKernelGGL((act_bwd16_kernel<T>), dim3((N + 511) / 512, groups), dim3(256), 0, st, static_cast<const T*>(dy), ldy,
+                       static_cast<const T*>(z), ldz, static_cast<T*>(dz), ldd, dbias ? ws : nullptr, M, N, act);
+    if (dbias)
+      hipLaunchKernelGGL((colsum16_join_kernel<T>), dim3((N + 63) / 64), dim3(1024), 0, st, ws, groups, N, static_cast<T*>(dbias));
+  };
+  if (dtype == T_BF16) go(__bf16{}); else go(_Float16{});
+  return check_launch("hopmi_act_bwd16");
+}

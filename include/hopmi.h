@@ -545,6 +545,51 @@ int hopmi_gemm_f16x2_tn_cs(const float* A, int lda, long long batch_stride_a, co
 int hopmi_gemm_split_ab(const void* Aimage, const void* Bimage, const float* bias, float* C, int M, int N, int K, int parts,
                         void* stream);
 
+/* ---- the trainable block's operators (csrc/layernorm.hip, linear16.hip, gradclip.hip): what fine-tuning the encoder or a residual block
+ *      next to it needs beside the frozen forms above.  dtype codes here: 0 = fp32, 1 = bf16, 2 = fp16; `ld*` are row strides in
+ *      ELEMENTS; data pointers need the alignment of one element, nothing more, unless a line says so.
+ *
+ * Layer normalisation, forward: y [M][D] dense = (x - mean) rstd * weight + bias over the last axis of x [M][ldx >= D]; weight and bias
+ * [D] of type wdtype (dtype, or 0 = fp32), either nullable; mean / rstd [M] fp32 for the backward (both or none).  Any D >= 1.
+ * Backward: dx [M][D] (nullable), dweight and dbias [D] of type wdtype (nullable), from dy [M][D] dense and the saved statistics.
+ * ws: hopmi_layernorm_bwd_ws_floats(M, D, dtype) floats when dweight or dbias is wanted (per-workgroup partial sums, added in index
+ * order by a second launch: bitwise reproducible). */
+int hopmi_layernorm_fwd(const void* x, long long ldx, const void* weight, const void* bias, int wdtype, void* y, float* mean, float* rstd,
+                        int M, int D, float eps, int dtype, void* stream);
+size_t hopmi_layernorm_bwd_ws_floats(int M, int D, int dtype);
+int hopmi_layernorm_bwd(const void* x, long long ldx, const void* dy, const float* mean, const float* rstd, const void* weight, int wdtype,
+                        void* dx, void* dweight, void* dbias, float* ws, int M, int D, int dtype, void* stream);
+
+/* Matrix product of 16-bit operands (dtype 1 or 2), fp32 accumulation, one rounding:
+ *     C [M][N] = act(A' B' + bias) + res        act: 0 none, 1 relu, 2 gelu (erf), 3 silu
+ * layout 0: A [M][K], B [N][K] (y = x w^T);  1: A [M][K], B [K][N] (dx = dz w);  2: A [K][M], B [K][N] (dw = dz^T x).  bias [N], res
+ * [M][ldr], z [M][ldz] nullable; z receives the values before the activation, rounded to dtype.  Operand rows have to start on 16 bytes
+ * and to be backed by whole 16-byte vectors, with ZEROS behind a row's last element where rows run along the contraction
+ * (hopmi_gemm16_direct says whether rows of `cols` elements are so by themselves; hopmi_pad16 copies rows into rows of ldp = a multiple
+ * of 8 elements, zeros behind the N-th) -- except with layout 0 and M <= 64, which takes any alignment.
+ * Operand strides up to 2^22 elements.  ws: hopmi_gemm16_ws_floats(M, N, K, layout) floats (contraction split over workgroups, added in
+ * split order by a second launch: bitwise reproducible). */
+size_t hopmi_gemm16_ws_floats(int M, int N, int K, int layout);
+int hopmi_gemm16_direct(const void* p, long long ld, int cols);
+int hopmi_gemm16(const void* A, long long lda, const void* B, long long ldb, int layout, void* C, long long ldc, const void* bias,
+                 const void* res, long long ldr, void* z, long long ldz, int act, int M, int N, int K, int dtype, float* ws, void* stream);
+int hopmi_pad16(const void* src, long long lds, void* dst, long long ldp, int M, int N, void* stream);
+/* dz [M][ldd] = dy act'(z), rows padded with zeros to 8 elements (nullable), and dbias [N] = the column sums of the unrounded dz
+ * (nullable; ws: hopmi_act_bwd16_ws_floats(M, N) floats, fixed summation order).  z [M][ldz >= N rounded up to 8], rows on 16 bytes;
+ * act 0 takes no z. */
+size_t hopmi_act_bwd16_ws_floats(int M, int N);
+int hopmi_act_bwd16(const void* dy, long long ldy, const void* z, long long ldz, void* dz, long long ldd, void* dbias, float* ws, int act,
+                    int M, int N, int dtype, void* stream);
+
+/* Global gradient norm and clipping: *norm (device, fp32) = the 2-norm over all `count` tensors, c = min(1, max_norm / (*norm + 1e-6)),
+ * and outs[t] = c grads[t]: outs NULL scales in place (nothing is written when c = 1), otherwise outs[t] is an fp32 tensor of the same
+ * numel.  grads / outs / numels / dtypes are HOST arrays, read before the call returns (the list travels in the kernels' arguments);
+ * at most 15 360 non-empty tensors.  Sums in 64 bits, in a fixed order.  A NaN or infinite norm scales by NaN or 0, as the formula
+ * says.  ws: hopmi_grad_clip_ws_bytes() bytes on 8. */
+size_t hopmi_grad_clip_ws_bytes(void);
+int hopmi_grad_clip(const void* const* grads, void* const* outs, const long long* numels, const int* dtypes, int count, float max_norm,
+                    float* norm, void* ws, void* stream);
+
 /* ---- log-mel spectrogram of the audio clips: data_loader/lmdb_data_loader.py:216-218
  *      melspec = librosa.feature.melspectrogram(y, sr=16000, n_fft=1024, hop_length=hop, power=2)   (librosa 0.8.1:
  *      periodic Hann window, center=True with reflect padding, Slaney mel filters);  out = power_to_db(melspec, ref=np.max).T
