@@ -2392,111 +2392,32 @@ def gru_bidirectional(x: torch.Tensor, gru: torch.nn.GRU, dropout_p: float = 0.0
 
 
 # ------------------------------------------------------------------- the trainable block's operators (layernorm / linear16 / gradclip)
-_DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}          # dtype codes of these entry points
+# Checks, autograd and the calls of the C ABI are in csrc/block_torch.cpp (_block.so): at these operators' sizes the host's share counts.
 _ACT = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
+_BLOCK = None
 
 
-def _refuse(msg):
-    raise _lib.HopmiError("hopmi: " + msg)
-
-
-def _same_device(first, *named):
-    """Refuses host tensors and tensors of different devices."""
-    dev = first.device
-    if not first.is_cuda:
-        _refuse(f"the operand is on {dev}; these operators only run on a ROCm device (no CPU fallback)")
-    for name, t in named:
-        if t is not None and t.device != dev:
-            _refuse(f"`{name}` is on {t.device}, the first operand on {dev}")
-    return dev
-
-
-def _rows(t, width):
-    """`t` (..., width) as rows: (a 2-d view or, where its rows do not lie at one stride, a dense copy; the row stride in elements)."""
-    if t.numel() >= width << 31:
-        _refuse(f"a tensor of shape {tuple(t.shape)} has 2^31 rows or more")
-    if t.is_contiguous():
-        return t.view(-1, width), width
-    t2 = t.reshape(-1, width)
-    if (width > 1 and t2.stride(1) != 1) or (t2.shape[0] > 1 and t2.stride(0) < width):
-        t2 = t2.contiguous()
-    return t2, (t2.stride(0) if t2.shape[0] > 1 else width)
-
-
-def _ln_forward(x2, ldx, weight, bias, eps, shape, keep):
-    M, D = x2.shape
-    y = torch.empty(shape, dtype=x2.dtype, device=x2.device)
-    stat = torch.empty(2, M, dtype=torch.float32, device=x2.device) if keep else None
-    if M:
-        sp = stat.data_ptr() if keep else 0
-        w = weight if weight is not None else bias
-        _lib.check(_timed("layernorm_fwd", 2 * x2.numel() * x2.element_size(), 8 * x2.numel(),
-                          lambda: _lib.lib().hopmi_layernorm_fwd(x2.data_ptr(), ldx, _ptr(weight), _ptr(bias), _DT[(x2 if w is None else w).dtype],
-                                                                 y.data_ptr(), sp or None, sp + 4 * M if keep else None, M, D, eps,
-                                                                 _DT[x2.dtype], _stream())), "hopmi_layernorm_fwd")
-    return y, stat
-
-
-class _LayerNormFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        x2, ldx = _rows(x, x.shape[-1])
-        y, stat = _ln_forward(x2, ldx, weight, bias, eps, x.shape, True)
-        ctx.save_for_backward(x, weight, bias, stat)
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        x, weight, bias, stat = ctx.saved_tensors
-        D = x.shape[-1]
-        x2, ldx = _rows(x, D)
-        dy = dy.contiguous()
-        M = x2.shape[0]
-        need_x, need_w, need_b, _ = ctx.needs_input_grad
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
-        new = torch.empty_like if M else torch.zeros_like
-        dw = new(weight) if need_w else None
-        db = new(bias) if need_b else None
-        if M:
-            L, code = _lib.lib(), _DT[x.dtype]
-            ws = torch.empty(L.hopmi_layernorm_bwd_ws_floats(M, D, code), dtype=torch.float32, device=x.device) if need_w or need_b else None
-            sp = stat.data_ptr()
-            w = weight if weight is not None else bias
-            _lib.check(_timed("layernorm_bwd", 3 * x2.numel() * x2.element_size(), 14 * x2.numel(),
-                              lambda: L.hopmi_layernorm_bwd(x2.data_ptr(), ldx, dy.data_ptr(), sp, sp + 4 * M, _ptr(weight),
-                                                            _DT[(x if w is None else w).dtype], _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), M, D,
-                                                            code, _stream())), "hopmi_layernorm_bwd")
-        return dx, dw, db, None
+def _block():
+    global _BLOCK
+    if _BLOCK is None:
+        _lib.lib()                                   # (the library itself first: its absence has a message of its own)
+        try:
+            from . import _block as mod
+        except ImportError as e:
+            raise _lib.HopmiError(f"hopmi: the torch side of the trainable block's operators is not built or does not load ({e}). "
+                                  "Run `python -c 'import __graft_entry__ as g; g.build()'`.") from e
+        mod.init(_lib._LIB_PATH, _lib.HopmiError)
+        _BLOCK = mod
+    return _BLOCK
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """torch.nn.functional.layer_norm over the last axis, with gradients for x, weight and bias (hopmi_layernorm_fwd / _bwd).
 
-    x (..., D): fp32, bf16 or fp16, any D >= 1, rows at any stride; weight, bias (D,) or None: x's type or fp32.  The output has x's type
-    and is dense; statistics and sums are fp32; the weights' gradients are summed in a fixed order (the same bits every time) and returned
-    in the weights' type.  Autocast does not change the types: what comes in decides."""
-    D = x.shape[-1] if x.dim() else 0
-    if D < 1 or x.dtype not in _DT:
-        _refuse(f"layer_norm: x has shape {tuple(x.shape)} and type {x.dtype} (fp32, bf16 or fp16 with a last axis of at least 1)")
-    dev = _same_device(x, ("weight", weight), ("bias", bias))
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None and (t.shape != (D,) or t.dtype not in (x.dtype, torch.float32)):
-            _refuse(f"layer_norm: `{name}` has shape {tuple(t.shape)} and type {t.dtype}; x's last axis is {D}, its type {x.dtype} (that type, or fp32)")
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        _refuse(f"layer_norm: weight is {weight.dtype} and bias {bias.dtype}: one type for both")
-    eps = float(eps)
-    if not eps >= 0.0:
-        _refuse(f"layer_norm: eps={eps}")
-    if dev.index != torch.cuda.current_device():
-        with torch.cuda.device(dev):
-            return layer_norm(x, weight, bias, eps)
-    weight = weight if weight is None or weight.is_contiguous() else weight.contiguous()
-    bias = bias if bias is None or bias.is_contiguous() else bias.contiguous()
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
-        return _LayerNormFn.apply(x, weight, bias, eps)
-    x2, ldx = _rows(x, D)
-    return _ln_forward(x2, ldx, weight, bias, eps, x.shape, False)[0]
+    x (..., D): fp32, bf16 or fp16, any D >= 1, rows at any stride; weight, bias (D,) or None: x's type or fp32, one type for both.  The
+    output has x's type and is dense; statistics and sums are fp32; the weights' gradients are summed in a fixed order (the same bits
+    every time) and returned in the weights' type.  Differentiable once.  Autocast does not change the types: what comes in decides."""
+    return (_BLOCK or _block()).layer_norm(x, weight, bias, eps)
 
 
 class LayerNorm(torch.nn.LayerNorm):
@@ -2505,105 +2426,10 @@ class LayerNorm(torch.nn.LayerNorm):
     def __init__(self, *args, **kwargs):
         super().__init__(*args, **kwargs)
         if len(self.normalized_shape) != 1:
-            _refuse(f"LayerNorm: normalized_shape={tuple(self.normalized_shape)}: one axis, the last")
+            raise _lib.HopmiError(f"hopmi: LayerNorm: normalized_shape={tuple(self.normalized_shape)}: one axis, the last")
 
     def forward(self, x):
         return layer_norm(x, self.weight, self.bias, self.eps)
-
-
-def _pad16(t2, ld):
-    """Rows copied to rows of whole 16-byte vectors, zeros behind the last element."""
-    M, N = t2.shape
-    ldp = (N + 7) // 8 * 8
-    out = torch.empty(M, ldp, dtype=t2.dtype, device=t2.device)
-    _lib.check(_lib.lib().hopmi_pad16(t2.data_ptr(), ld, out.data_ptr(), ldp, M, N, _stream()), "hopmi_pad16")
-    return out, ldp
-
-
-def _operand16(t2, ld):
-    """(tensor, row stride) as hopmi_gemm16 takes it: as it is where its rows start and end on 16 bytes, else a padded copy."""
-    if t2.data_ptr() & 15 or ld & 7 or t2.shape[1] & 7 or ld > 1 << 22:
-        return _pad16(t2, ld)
-    return t2, ld
-
-
-def _gemm16(a, lda, b, ldb, layout, out, M, N, K, bias=None, res=None, ldr=0, z=None, act=0):
-    L = _lib.lib()
-    nws = L.hopmi_gemm16_ws_floats(M, N, K, layout)
-    ws = torch.empty(nws, dtype=torch.float32, device=out.device) if nws else None
-    e = out.element_size()
-    _lib.check(_timed("gemm16", e * (M * K + N * K + (1 + (res is not None)) * M * N), 2 * M * N * K,
-                      lambda: L.hopmi_gemm16(a.data_ptr(), lda, b.data_ptr(), ldb, layout, out.data_ptr(), N, _ptr(bias), _ptr(res), ldr,
-                                             _ptr(z), 0 if z is None else z.shape[1], act, M, N, K, _DT[out.dtype], _ptr(ws), _stream())),
-               "hopmi_gemm16")
-
-
-_FEW_ROWS16 = 64                 # up to here layout 0 takes operands of any alignment
-
-
-def _linear_act_forward(x2, ldx, w, ldw, bias, res, act, shape, keep_z):
-    M, K = x2.shape
-    N = w.shape[0]
-    y = torch.empty(shape, dtype=x2.dtype, device=x2.device)
-    z = torch.empty(M, (N + 7) // 8 * 8, dtype=x2.dtype, device=x2.device) if keep_z else None
-    if M:
-        r2, ldr = (None, 0) if res is None else _rows(res, N)
-        if M > _FEW_ROWS16:
-            x2, ldx = _operand16(x2, ldx)
-            w, ldw = _operand16(w, ldw)
-        _gemm16(x2, ldx, w, ldw, 0, y, M, N, K, bias, r2, ldr, z, act)
-    return y, z, x2, w
-
-
-class _LinearActFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, w, bias, res, act):
-        K = x.shape[-1]
-        x2, ldx = _rows(x, K)
-        w2, ldw = _rows(w, K)
-        need_z = act != 0 and any(ctx.needs_input_grad[:3])
-        y, z, xp, wp = _linear_act_forward(x2, ldx, w2, ldw, bias, res, act, x.shape[:-1] + (w.shape[0],), need_z)
-        # (padded copies, where the forward had to make them, serve the backward's products too)
-        ctx.padded = (xp if xp is not x2 else None, wp if wp is not w2 else None)
-        ctx.save_for_backward(x, w, z)
-        ctx.act = act
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        x, w, z = ctx.saved_tensors
-        need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
-        N, K = w.shape
-        act, dx, dw, db = ctx.act, None, None, None
-        if need_x or need_w or need_b:
-            g, ldg = _rows(dy, N)
-            M = g.shape[0]
-            new = torch.empty if M else torch.zeros
-            dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
-            dw = new(N, K, dtype=w.dtype, device=w.device) if need_w else None
-            db = new(N, dtype=w.dtype, device=w.device) if need_b else None
-            if M:
-                products = need_x or need_w
-                plain = act == 0 and not (g.data_ptr() & 15 or ldg & 7 or N & 7 or ldg > 1 << 22)      # dz is dy as it lies there
-                dz, ldz = (g, ldg) if plain else (None, 0)
-                if (products and not plain) or need_b:
-                    L = _lib.lib()
-                    if products and not plain:
-                        ldz = (N + 7) // 8 * 8
-                        dz = torch.empty(M, ldz, dtype=g.dtype, device=g.device)
-                    ws = torch.empty(L.hopmi_act_bwd16_ws_floats(M, N), dtype=torch.float32, device=g.device) if need_b else None
-                    _lib.check(_timed("act_bwd16", 2 * M * N * (1 + (z is not None) + (dz is not g)), 16 * M * N,
-                                      lambda: L.hopmi_act_bwd16(g.data_ptr(), ldg, _ptr(z), 0 if z is None else z.shape[1],
-                                                                None if plain else _ptr(dz), ldz, _ptr(db), _ptr(ws), act, M, N,
-                                                                _DT[g.dtype], _stream())), "hopmi_act_bwd16")
-                if need_x:
-                    wp, ldw = (ctx.padded[1], ctx.padded[1].shape[1]) if ctx.padded[1] is not None else _operand16(*_rows(w, K))
-                    _gemm16(dz, ldz, wp, ldw, 1, dx, M, K, N)
-                if need_w:
-                    xp, ldx = (ctx.padded[0], ctx.padded[0].shape[1]) if ctx.padded[0] is not None else _operand16(*_rows(x, K))
-                    _gemm16(dz, ldz, xp, ldx, 2, dw, N, K, M)
-        return dx, dw, db, dy if need_r else None, None
 
 
 def linear_act(x, w, bias=None, residual=None, activation="none"):
@@ -2613,50 +2439,12 @@ def linear_act(x, w, bias=None, residual=None, activation="none"):
     to its type first; fp32 products are `linear`'s).  activation: "none", "relu", "gelu" (erf) or "silu".  Accumulation, bias,
     activation and residual are fp32, with one rounding at the end.  Any sizes >= 1, strides and alignments; one to 64 rows take a form
     that reads w once.  For the backward pass the values before the activation are kept in the operands' type, and dz = dy act'(z) is
-    rounded to it once, in front of the two products; the bias gradient sums the unrounded dz.  No atomics: the same bits every time."""
-    if activation not in _ACT:
-        _refuse(f"linear_act: activation={activation!r} (one of {', '.join(_ACT)})")
-    if torch.is_autocast_enabled("cuda"):
-        dt = torch.get_autocast_dtype("cuda")
-        x, w, bias, residual = (t if t is None or t.dtype == dt else t.to(dt) for t in (x, w, bias, residual))
-    dev = _same_device(x, ("w", w), ("bias", bias), ("residual", residual))
-    if x.dtype not in (torch.bfloat16, torch.float16):
-        _refuse(f"linear_act: x is {x.dtype}: bf16 or fp16 (fp32 products: ops.linear)")
-    for name, t in (("w", w), ("bias", bias), ("residual", residual)):
-        if t is not None and t.dtype != x.dtype:
-            _refuse(f"linear_act: `{name}` is {t.dtype}, x {x.dtype}: one type for all operands")
-    if x.dim() < 1 or w.dim() != 2 or w.shape[1] != x.shape[-1] or w.shape[0] < 1 or w.shape[1] < 1:
-        _refuse(f"linear_act: x {tuple(x.shape)} and w {tuple(w.shape)} (N, K) do not fit, or have an empty side")
-    N, K = w.shape
-    shape = x.shape[:-1] + (N,)
-    if bias is not None and bias.shape != (N,):
-        _refuse(f"linear_act: bias has shape {tuple(bias.shape)}, w {tuple(w.shape)}")
-    if residual is not None and residual.shape != shape:
-        try:
-            residual = residual.expand(shape)
-        except RuntimeError:
-            _refuse(f"linear_act: residual of shape {tuple(residual.shape)} does not broadcast to {tuple(shape)}")
-    if dev.index != torch.cuda.current_device():
-        with torch.cuda.device(dev):
-            return linear_act(x, w, bias, residual, activation)
-    bias = bias if bias is None or bias.is_contiguous() else bias.contiguous()
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w, bias, residual)):
-        return _LinearActFn.apply(x, w, bias, residual, _ACT[activation])
-    x2, ldx = _rows(x, K)
-    w2, ldw = _rows(w, K)
-    return _linear_act_forward(x2, ldx, w2, ldw, bias, residual, _ACT[activation], shape, False)[0]
-
-
-def _dense(t):
-    """Does the tensor fill one stretch of memory, each place once (in whatever order of its axes)?"""
-    if t.is_contiguous():
-        return True
-    want = 1
-    for st, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
-        if st != want:
-            return False
-        want *= n
-    return True
+    rounded to it once, in front of the two products; the bias gradient sums the unrounded dz.  No atomics: the same bits every time.
+    Differentiable once."""
+    act = _ACT.get(activation)
+    if act is None:
+        raise _lib.HopmiError(f"hopmi: linear_act: activation={activation!r} (one of {', '.join(_ACT)})")
+    return (_BLOCK or _block()).linear_act(x, w, bias, residual, act)
 
 
 class GradClip:
@@ -2666,54 +2454,12 @@ class GradClip:
     the clipped values (what hopmi_adam_multi reads, from 16-bit gradients) while the gradients stay as they are."""
 
     def __init__(self, tensors, out=None):
-        import ctypes
-        self.tensors = list(tensors)
-        self.out = None if out is None else list(out)
-        if not self.tensors:
-            _refuse("GradClip: an empty list of tensors")
-        if self.out is not None and len(self.out) != len(self.tensors):
-            _refuse(f"GradClip: {len(self.out)} outputs for {len(self.tensors)} tensors")
-        self.device = _same_device(self.tensors[0], *((f"tensors[{i}]", t) for i, t in enumerate(self.tensors)),
-                                   *((f"out[{i}]", t) for i, t in enumerate(self.out or ())))
-        spans = []
-        for i, t in enumerate(self.tensors):
-            if t.layout != torch.strided or t.dtype not in _DT or not _dense(t):
-                _refuse(f"GradClip: tensors[{i}] ({t.dtype}, shape {tuple(t.shape)}, strides {t.stride() if t.layout == torch.strided else t.layout}) "
-                        "is not an fp32, bf16 or fp16 tensor without gaps (.contiguous() makes one)")
-            spans.append((t.data_ptr(), t.numel() * t.element_size(), f"tensors[{i}]"))
-        for i, (t, o) in enumerate(zip(self.tensors, self.out or ())):
-            if o.layout != torch.strided or o.dtype != torch.float32 or o.shape != t.shape or (t.numel() > 1 and o.stride() != t.stride()):
-                _refuse(f"GradClip: out[{i}] is not an fp32 tensor of tensors[{i}]'s shape and strides")
-            spans.append((o.data_ptr(), o.numel() * 4, f"out[{i}]"))
-        spans = sorted(s for s in spans if s[1])
-        for (p, n, a), (q, _, b) in zip(spans, spans[1:]):
-            if p + n > q:
-                _refuse(f"GradClip: {a} and {b} share memory")
-        n = len(self.tensors)
-        self._in = (ctypes.c_void_p * n)(*[t.data_ptr() for t in self.tensors])
-        self._out = None if self.out is None else (ctypes.c_void_p * n)(*[t.data_ptr() for t in self.out])
-        self._n = (ctypes.c_longlong * n)(*[t.numel() for t in self.tensors])
-        self._dt = (ctypes.c_int * n)(*[_DT[t.dtype] for t in self.tensors])
-        self._elements = sum(self._n)
+        self._plan = _block().ClipPlan(list(tensors), None if out is None else list(out))
 
-    @torch.no_grad()
     def clip_(self, max_norm):
         """Scales the gradients by min(1, max_norm / (norm + 1e-6)) and returns their 2-norm before that, an fp32 scalar on the device
         (nothing is read back).  max_norm=inf gives the norm and leaves in-place gradients as they are."""
-        max_norm = float(max_norm)
-        if not max_norm >= 0.0:
-            _refuse(f"GradClip: max_norm={max_norm}")
-        if self.device.index != torch.cuda.current_device():
-            with torch.cuda.device(self.device):
-                return self.clip_(max_norm)
-        L = _lib.lib()
-        norm = torch.empty((), dtype=torch.float32, device=self.device)
-        ws = torch.empty(L.hopmi_grad_clip_ws_bytes(), dtype=torch.uint8, device=self.device)
-        _lib.check(_timed("grad_clip", 4 * self._elements, 3 * self._elements,
-                          lambda: L.hopmi_grad_clip(self._in, self._out, self._n, self._dt, len(self.tensors), max_norm, norm.data_ptr(),
-                                                    ws.data_ptr(), _stream())), "hopmi_grad_clip")
-        torch.autograd.graph.increment_version(self.tensors if self.out is None else self.out)     # (written behind autograd's back)
-        return norm
+        return self._plan.clip(max_norm)
 
 
 def clip_grad_norm_(parameters, max_norm):

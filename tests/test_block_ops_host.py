@@ -36,20 +36,6 @@ def test_host_tensors_and_bad_arguments_are_refused():
     assert list(ops.LayerNorm(8).state_dict()) == list(torch.nn.LayerNorm(8).state_dict())
 
 
-def test_dense_says_which_tensors_fill_their_memory():
-    t = torch.zeros(4, 6, 5)
-    assert ops._dense(t) and ops._dense(t.permute(2, 0, 1)) and ops._dense(t[1]) and ops._dense(t[:, :, :0]) and ops._dense(torch.zeros(1, 3)[:, 1:2])
-    assert not ops._dense(t[:, 1]) and not ops._dense(t[..., ::2]) and not ops._dense(torch.zeros(3, 1).expand(3, 4))
-
-
-def test_rows_keeps_one_stride_and_copies_what_has_none():
-    t = torch.zeros(4, 6, 5)
-    assert ops._rows(t, 5)[1] == 5 and ops._rows(t[..., 1:4], 3)[1] == 5 and ops._rows(t[..., 1:4], 3)[0].data_ptr() == t[..., 1:4].data_ptr()
-    assert ops._rows(t.transpose(1, 2), 6)[1] == 6                      # last axis not contiguous: a copy
-    assert ops._rows(torch.zeros(5).expand(7, 5), 5)[1] == 5             # rows on top of one another: a copy
-    assert ops._rows(t[:0], 5)[0].shape == (0, 5)
-
-
 def test_layernorm_entry_points_refuse():
     L = _lib.lib()
     args = lambda dt=0, wdt=0, M=4, D=8, ld=8, eps=1e-5, x=ONE: L.hopmi_layernorm_fwd(x, ld, ONE, ONE, wdt, ONE, None, None, M, D, eps, dt, None)

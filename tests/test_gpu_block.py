@@ -371,6 +371,27 @@ def test_linear_act_refusals_on_device():
         assert y.dtype == torch.bfloat16 and torch.autograd.grad(y.sum(), xf)[0].dtype == torch.float32
 
 
+def test_gradients_of_gradients_are_refused_where_they_are_taken():
+    """Under create_graph the first gradients are right; going through them again is an error, not a silent zero."""
+    g = _rng(13)
+    x, w = _randn(g, 80, 24).requires_grad_(), _randn(g, 24).requires_grad_()
+    y = ops.layer_norm(x, w)
+    first = torch.autograd.grad(y.sum(), [x, w], create_graph=True)
+    assert all(torch.equal(p, q) for p, q in zip(first, torch.autograd.grad(ops.layer_norm(x, w).sum(), [x, w])))
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(first[0].square().sum(), x)
+    xb, wb = x.detach().bfloat16().requires_grad_(), _randn(g, 16, 24).bfloat16().requires_grad_()
+    gb = torch.autograd.grad(ops.linear_act(xb, wb, activation="gelu").sum(), [xb, wb], create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(gb[0].float().square().sum(), xb)
+    # an operand changed between the passes is noticed
+    y = ops.layer_norm(x, w)
+    with torch.no_grad():
+        w.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y.sum(), x)
+
+
 # ------------------------------------------------------------------------------------------------------------ GradClip
 def _clip_case(seed, count, dtypes, scale=1.0, odd=True):
     g = _rng(seed)
