@@ -76,18 +76,26 @@ __device__ __forceinline__ float act_grad(float z, int act) {
   return 1.f;
 }
 
-// four consecutive elements at any element address
-template <typename T> __device__ __forceinline__ void ld4f(const T* p, float (&f)[4]) {
-  const u32x2_any v = *reinterpret_cast<const u32x2_any*>(p);
-  const u32x4_t w = {v[0], v[1], 0, 0};
+// V (4 or 8) consecutive elements at any element address
+template <typename T, int V> __device__ __forceinline__ void ldv(const T* p, float (&f)[V]) {
+  u32x4_t w = {0, 0, 0, 0};
+  if constexpr (V == 8) w = ld16(p);
+  else {
+    const u32x2_any v = *reinterpret_cast<const u32x2_any*>(p);
+    w[0] = v[0];
+    w[1] = v[1];
+  }
 #pragma unroll
-  for (int e = 0; e < 4; ++e) f[e] = vget(w, e, p);
+  for (int e = 0; e < V; ++e) f[e] = vget(w, e, p);
 }
-template <typename T> __device__ __forceinline__ void st4f(T* p, const float (&f)[4]) {
-  u32x2_any v;
-  v[0] = pk2(f[0], f[1], p);
-  v[1] = pk2(f[2], f[3], p);
-  *reinterpret_cast<u32x2_any*>(p) = v;
+template <typename T, int V> __device__ __forceinline__ void stv(T* p, const float (&f)[V]) {
+  if constexpr (V == 8) st16(p, vpack(f, p));
+  else {
+    u32x2_any v;
+    v[0] = pk2(f[0], f[1], p);
+    v[1] = pk2(f[2], f[3], p);
+    *reinterpret_cast<u32x2_any*>(p) = v;
+  }
 }
 
 template <typename T> struct Epi16 {
@@ -98,37 +106,52 @@ template <typename T> struct Epi16 {
                                  // loses by it is a third of what the rounding of dz itself loses)
   int act;
 };
-// columns col .. col + 3 of a row, of which `left` (>= 1) exist
-template <typename T> __device__ __forceinline__ void epilogue4(const Epi16<T>& E, long long row, int col, int left, float (&f)[4]) {
-  float t[4];
-  if (left >= 4) {
-    if (E.bias != nullptr) {
-      ld4f(E.bias + col, t);
+// columns col .. col + V - 1 of a row, of which `left` (>= 1) exist
+template <int V, typename T> __device__ __forceinline__ void epilogue16(const Epi16<T>& E, long long row, int col, int left, float (&f)[V]) {
+  const bool whole = left >= V;
+  float b[V], r[V];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) f[e] += t[e];
+  for (int e = 0; e < V; ++e) b[e] = r[e] = 0.f;
+  if (E.bias != nullptr) {
+    if (whole) ldv(E.bias + col, b);
+    else {
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (e < left) b[e] = to_f(E.bias[col + e]);
     }
-    if (E.z != nullptr) st4f(E.z + row * E.ldz + col, f);
-    if (E.act != ACT_NONE) {
+  }
+  if (E.res != nullptr) {
+    const T* p = E.res + row * E.ldr + col;
+    if (whole) ldv(p, r);
+    else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) f[e] = act_fwd(f[e], E.act);
+      for (int e = 0; e < V; ++e)
+        if (e < left) r[e] = to_f(p[e]);
     }
-    if (E.res != nullptr) {
-      ld4f(E.res + row * E.ldr + col, t);
+  }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) f[e] += t[e];
+  for (int e = 0; e < V; ++e) f[e] += b[e];
+  if (E.z != nullptr) {
+    T* p = E.z + row * E.ldz + col;
+    if (whole) stv(p, f);
+    else {
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (e < left) p[e] = (T)f[e];
     }
-    st4f(E.C + row * E.ldc + col, f);
-  } else {
+  }
+  if (E.act != ACT_NONE) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (e < left) {
-        float v = f[e];
-        if (E.bias != nullptr) v += to_f(E.bias[col + e]);
-        if (E.z != nullptr) E.z[row * E.ldz + col + e] = (T)v;
-        v = act_fwd(v, E.act);
-        if (E.res != nullptr) v += to_f(E.res[row * E.ldr + col + e]);
-        E.C[row * E.ldc + col + e] = (T)v;
-      }
+    for (int e = 0; e < V; ++e) f[e] = act_fwd(f[e], E.act);
+  }
+#pragma unroll
+  for (int e = 0; e < V; ++e) f[e] += r[e];
+  T* p = E.C + row * E.ldc + col;
+  if (whole) stv(p, f);
+  else {
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (e < left) p[e] = (T)f[e];
   }
 }
 
@@ -141,72 +164,70 @@ template <typename T> struct Gemm16 {
   int tiles_m, tiles_n, splits;
 };
 
-constexpr int G16_BK = 64;       // contraction per step
+constexpr int G16_BK = 32;       // contraction per step: one MFMA's
 
-// Staging of one operand's tile of R rows (KC: [R][64], else [64][R]) by NW waves, and its fragments.
+// Staging of one operand's tile of R rows (KC: [R][32], else [32][R]) by NW waves, and its fragments.
 template <typename T, int R, int NW, bool KC> struct Tile16 {
-  static constexpr int NI = R / 8 / NW;            // 1 KiB DMA instructions per wave and step
-  static constexpr int LPR = KC ? 8 : R / 8;       // lanes per tile row in memory order
+  static constexpr int BK = G16_BK, BYTES = R * BK * 2;
+  static constexpr int NI = BYTES / 1024 / NW;     // 1 KiB DMA instructions per wave and step
+  static constexpr int CPR = BK / 8;               // 16-byte chunks per row (KC)
+  static constexpr int LPR = KC ? CPR : R / 8;     // lanes per tile row in memory order
   const char* base;                                // uniform; advances by one step
   long long adv;
   unsigned off[NI];                                // this lane's bytes from base
-  int kk[NI];                                      // contraction index (within a step) of this lane's first element
 
   __device__ __forceinline__ void init(const T* p, long long ld, int r0, int r_total, int k0, int lane, int wave) {
-    if (KC) {
-      base = reinterpret_cast<const char*>(p + (long long)r0 * ld + k0);
-      adv = G16_BK * 2;
-    } else {
-      base = reinterpret_cast<const char*>(p + (long long)k0 * ld + r0);
-      adv = G16_BK * 2 * ld;
-    }
+    base = reinterpret_cast<const char*>(KC ? p + (long long)r0 * ld + k0 : p + (long long)k0 * ld + r0);
+    adv = KC ? BK * 2 : BK * 2 * ld;
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
+      const int row = (i * NW + wave) * (64 / LPR) + lane / LPR, s = lane % LPR;
       if (KC) {
-        const int row = (i * NW + wave) * 8 + (lane >> 3), c = (lane & 7) ^ ((row >> 1) & 7);
         const int rc = min(row, r_total - 1 - r0);             // (r_total > r0)
-        off[i] = (unsigned)(rc * ld * 2 + c * 16);
-        kk[i] = c * 8;
+        off[i] = (unsigned)(rc * ld * 2 + (s ^ ((row >> 2) & 3)) * 16);
       } else {
-        const int k = (i * NW + wave) * (64 / LPR) + lane / LPR, s = lane % LPR;
-        const int c = ((((s >> 1) ^ ((k & 3) | ((k >> 3) & 1) << 2)) << 1) | (s & 1)) * 8;
+        const int c = ((((s >> 1) ^ ((row & 3) | ((row >> 3) & 1) << 2)) << 1) | (s & 1)) * 8;
         const int cc = min(c, ((r_total - r0 + 7) & ~7) - 8);  // (whole chunks: the operand's rows are padded to 8)
-        off[i] = (unsigned)(k * ld * 2 + cc * 2);
-        kk[i] = k;
+        off[i] = (unsigned)(row * ld * 2 + cc * 2);
       }
     }
   }
-  // issues the step's DMA into `lds`; `left`: contraction indices that exist from this step's start on (KC: rounded up to 8)
-  __device__ __forceinline__ void load(char* lds, int left, int wave) {
-    if (left >= G16_BK) {
+  // issues a whole step's DMA into `lds`
+  __device__ __forceinline__ void load(char* lds, int wave) {
+#ifdef __HIP_DEVICE_COMPILE__                      // (the host pass has no such type)
+    const __amdgpu_buffer_rsrc_t src = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, -1, 0x00020000);
 #pragma unroll
-      for (int i = 0; i < NI; ++i)
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(base + off[i]),
-                                         (__attribute__((address_space(3))) void*)(lds + (i * NW + wave) * 1024), 16, 0, 0);
-    } else {
+    for (int i = 0; i < NI; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (__attribute__((address_space(3))) void*)(lds + (i * NW + wave) * 1024), 16, off[i], 0, 0, 0);
+#endif
+    base += adv;
+  }
+  // ... of a step of which only `left` contraction indices exist (KC: rounded up to 8); zeros behind them
+  __device__ __forceinline__ void load_edge(char* lds, int left, int lane, int wave) {
 #pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        const char* src = kk[i] < left ? base + off[i] : reinterpret_cast<const char*>(g_zero16);
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
-                                         (__attribute__((address_space(3))) void*)(lds + (i * NW + wave) * 1024), 16, 0, 0);
-      }
+    for (int i = 0; i < NI; ++i) {
+      const int row = (i * NW + wave) * (64 / LPR) + lane / LPR;
+      const int k = KC ? ((lane % LPR) ^ ((row >> 2) & 3)) * 8 : row;
+      const char* src = k < left ? base + off[i] : reinterpret_cast<const char*>(g_zero16);
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
+                                       (__attribute__((address_space(3))) void*)(lds + (i * NW + wave) * 1024), 16, 0, 0);
     }
     base += adv;
   }
 };
 
-// fragments of NB 16-row blocks starting at block `b0` of a staged tile, contraction half ks
+// fragments of NB 16-row blocks starting at block `b0` of a staged tile
 template <typename T, int R, int NB, bool KC>
-__device__ __forceinline__ void frags16(const char* lds, int b0, int ks, int n, int q, u32x4_t (&f)[NB]) {
+__device__ __forceinline__ void frags16(const char* lds, int b0, int n, int q, u32x4_t (&f)[NB]) {
   if (KC) {
-    const char* p = lds + b0 * 2048 + n * 128 + (((ks * 4 + q) ^ (n >> 1)) << 4);
+    const char* p = lds + (b0 * 16 + n) * 64 + ((q ^ (n >> 2)) << 4);
 #pragma unroll
-    for (int j = 0; j < NB; ++j) f[j] = *reinterpret_cast<const u32x4_t*>(p + j * 2048);
+    for (int j = 0; j < NB; ++j) f[j] = *reinterpret_cast<const u32x4_t*>(p + j * 1024);
   } else {
     typedef short s4 __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) s4* s4p;
     const int sw = (n >> 2) | (q & 1) << 2;
-    const char* p = lds + (ks * 32 + 8 * q + (n >> 2)) * (R * 2) + (n & 3) * 8;
+    const char* p = lds + (8 * q + (n >> 2)) * (R * 2) + (n & 3) * 8;
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
       const char* a = p + (((b0 + j) ^ sw) << 5);
@@ -218,10 +239,24 @@ __device__ __forceinline__ void frags16(const char* lds, int b0, int ks, int n, 
   }
 }
 
-template <typename T, int BM, int BN, int WR, int WC, bool KA, bool KB>
-__global__ __launch_bounds__(64 * WR * WC) void gemm16_kernel(Gemm16<T> G) {
-  constexpr int NW = WR * WC, RB = BM / WR / 16, CB = BN / WC / 16;
-  constexpr int SA = BM * G16_BK * 2, SB = BN * G16_BK * 2, ST = SA + SB;
+// s_waitcnt vmcnt(N) lgkmcnt(0), as the builtin (the compiler's own counting then knows of it), and the barrier, with nothing moved across
+template <int N> __device__ __forceinline__ void wait_and_meet() {
+  static_assert(N < 64, "six bits");
+  __builtin_amdgcn_s_waitcnt((N & 15) | 7 << 4 | (N >> 4) << 14);
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// The steps are pipelined twice: ST LDS buffers of one step each, filled by DMA ST - 1 to ST steps ahead, and two sets of fragment
+// registers: a step's products run on fragments that were read during the step before, so neither the DMA nor the LDS reads are waited
+// for in a wave's own time.  One barrier per step.
+template <typename T, int BM, int BN, int WR, int WC, int ST, int OCC, bool KA, bool KB>
+__global__ __launch_bounds__(64 * WR * WC, OCC) void gemm16_kernel(Gemm16<T> G) {
+  constexpr int NW = WR * WC, RB = BM / WR / 16, CB = BN / WC / 16, BK = G16_BK;
+  using TA = Tile16<T, BM, NW, KA>;
+  using TB = Tile16<T, BN, NW, KB>;
+  constexpr int SB = TA::BYTES + TB::BYTES, NI = TA::NI + TB::NI;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, q = lane >> 4;
   const int wr = wave / WC, wc = wave % WC;
@@ -238,60 +273,112 @@ __global__ __launch_bounds__(64 * WR * WC) void gemm16_kernel(Gemm16<T> G) {
   const int per_group = 8 * G.tiles_n, g = id / per_group, first = g * 8, size = min(8, G.tiles_m - first);
   const int tm = first + (id - g * per_group) % size, tn = (id - g * per_group) / size;
   const int r0 = tm * BM, c0 = tn * BN;
-  const int steps = (G.K + G16_BK - 1) / G16_BK;
-  const int s0 = (int)((long long)steps * split / G.splits), s1 = (int)((long long)steps * (split + 1) / G.splits);
-  Tile16<T, BM, NW, KA> ta;
-  Tile16<T, BN, NW, KB> tb;
-  ta.init(G.A, G.lda, r0, G.M, s0 * G16_BK, lane, wave);
-  tb.init(G.B, G.ldb, c0, G.N, s0 * G16_BK, lane, wave);
-  const int ka = KA ? (G.K + 7) & ~7 : G.K, kb = KB ? (G.K + 7) & ~7 : G.K;
+  const int all = (G.K + BK - 1) / BK;
+  const int s0 = (int)((long long)all * split / G.splits), steps = (int)((long long)all * (split + 1) / G.splits) - s0;
+  TA ta;
+  TB tb;
+  ta.init(G.A, G.lda, r0, G.M, s0 * BK, lane, wave);
+  tb.init(G.B, G.ldb, c0, G.N, s0 * BK, lane, wave);
   f32x4 acc[RB][CB];
 #pragma unroll
   for (int i = 0; i < RB; ++i)
 #pragma unroll
     for (int j = 0; j < CB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  if (s0 < s1) {
-    ta.load(lds, ka - s0 * G16_BK, wave);
-    tb.load(lds + SA, kb - s0 * G16_BK, wave);
-  }
-  for (int s = s0; s < s1; ++s) {
-    char* cur = lds + ((s - s0) & 1) * ST;
-    // this step's tiles are in LDS once every wave's DMA is (vmcnt, then the barrier), and every wave is done with the other buffer
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    if (s + 1 < s1) {
-      char* nxt = lds + ((s + 1 - s0) & 1) * ST;
-      ta.load(nxt, ka - (s + 1) * G16_BK, wave);
-      tb.load(nxt + SA, kb - (s + 1) * G16_BK, wave);
+  auto load = [&](char* to) {
+    ta.load(to, wave);
+    tb.load(to + TA::BYTES, wave);
+  };
+  auto load_any = [&](char* to, int s) {           // step s of this workgroup, which may be the contraction's last
+    const int left = G.K - (s0 + s) * BK;
+    if (left >= BK) load(to);
+    else {
+      ta.load_edge(to, KA ? (left + 7) & ~7 : left, lane, wave);
+      tb.load_edge(to + TA::BYTES, KB ? (left + 7) & ~7 : left, lane, wave);
     }
+  };
+  u32x4_t fa0[RB], fb0[CB], fa1[RB], fb1[CB];
+  char* cur = lds;
+  auto advance = [&] { cur = cur + SB == lds + ST * SB ? lds : cur + SB; };
+  auto fetch = [&](u32x4_t (&a)[RB], u32x4_t (&b)[CB]) {
+    frags16<T, BM, RB, KA>(cur, wr * RB, n, q, a);
+    frags16<T, BN, CB, KB>(cur + TA::BYTES, wc * CB, n, q, b);
+  };
+  auto multiply = [&](const u32x4_t (&a)[RB], const u32x4_t (&b)[CB]) {
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      u32x4_t fa[RB], fb[CB];
-      frags16<T, BM, RB, KA>(cur, wr * RB, ks, n, q, fa);
-      frags16<T, BN, CB, KB>(cur + SA, wc * CB, ks, n, q, fb);
+    for (int i = 0; i < RB; ++i)
 #pragma unroll
-      for (int i = 0; i < RB; ++i)
+      for (int j = 0; j < CB; ++j) acc[i][j] = mfma16x32(b[j], a[i], acc[i][j], G.A);
+    constexpr int NR = (KA ? RB : 2 * RB) + (KB ? CB : 2 * CB), PER = RB * CB / NR > 0 ? RB * CB / NR : 1;
 #pragma unroll
-        for (int j = 0; j < CB; ++j) acc[i][j] = mfma16x32(fb[j], fa[i], acc[i][j], G.A);
+    for (int k = 0; k < NR; ++k) {                 // the reads spread between the products
+      __builtin_amdgcn_sched_group_barrier(0x008, PER, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
     }
+  };
+#pragma unroll
+  for (int s = 0; s < ST; ++s)
+    if (s < steps) load_any(lds + s * SB, s);
+  if (steps >= ST) wait_and_meet<NI * (ST - 1)>();
+  else wait_and_meet<0>();
+  fetch(fa0, fb0);
+  // Step s: step s + 1 is in LDS once every wave's DMA for it is (counted, then the barrier); every wave has its fragments of step s, so
+  // that buffer takes step s + ST.
+  int s = 0;
+  for (; s + ST + 2 < steps; s += 2) {             // (steps that load whole ones)
+    wait_and_meet<NI * (ST - 2)>();
+    load(cur);
+    advance();
+    fetch(fa1, fb1);
+    multiply(fa0, fb0);
+    wait_and_meet<NI * (ST - 2)>();
+    load(cur);
+    advance();
+    fetch(fa0, fb0);
+    multiply(fa1, fb1);
   }
-  const int row0 = r0 + wr * RB * 16 + n, col0 = c0 + wc * CB * 16 + 4 * q;
+#pragma unroll 1
+  for (; s < steps; ++s) {                         // the last ST + 2 at most: the contraction's end may be among what they load
+    if (s + ST - 1 < steps) wait_and_meet<NI * (ST - 2)>();
+    else wait_and_meet<0>();
+    if (s + ST < steps) load_any(cur, s + ST);
+    advance();
+    fetch(fa1, fb1);                               // (past the last step: values that nothing uses)
+    multiply(fa0, fb0);
+#pragma unroll
+    for (int i = 0; i < RB; ++i) fa0[i] = fa1[i];
+#pragma unroll
+    for (int j = 0; j < CB; ++j) fb0[j] = fb1[j];
+  }
+  // The results leave through LDS, 16 rows of every wave at a time: eight consecutive columns per lane then, whole lines per wave, and one
+  // copy of the epilogue's code.  (The last reads of the buffers are awaited first; no DMA is in flight any more.)
+  constexpr int LDC = BN + 4, VR = BN / 8, ROWS = WR * 16;
+  static_assert(ROWS * LDC * 4 <= ST * SB, "the staged rows fit the buffers");
+  float* stage = reinterpret_cast<float*>(lds);
 #pragma unroll
   for (int i = 0; i < RB; ++i) {
-    const long long row = row0 + i * 16;
-    if (row >= G.M) continue;
+    __syncthreads();
 #pragma unroll
-    for (int j = 0; j < CB; ++j) {
-      const int col = col0 + j * 16, left = G.N - col;
-      if (left <= 0) continue;
-      float f[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+    for (int j = 0; j < CB; ++j) *reinterpret_cast<f32x4*>(&stage[(wr * 16 + n) * LDC + (wc * CB + j) * 16 + 4 * q]) = acc[i][j];
+    __syncthreads();
+#pragma unroll 1
+    for (int v = threadIdx.x; v < ROWS * VR; v += 64 * NW) {
+      const int sr = v / VR, col = c0 + v % VR * 8, left = G.N - col;
+      const long long row = r0 + (sr / 16 * RB + i) * 16 + sr % 16;
+      if (row >= G.M || left <= 0) continue;
+      const f32x4 lo = *reinterpret_cast<const f32x4*>(&stage[sr * LDC + v % VR * 8]), hi = *reinterpret_cast<const f32x4*>(&stage[sr * LDC + v % VR * 8 + 4]);
+      float f[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
       if (G.part != nullptr) {
         float* p = G.part + ((long long)split * G.M + row) * G.N + col;
-        if (left >= 4) *reinterpret_cast<u32x4_any*>(p) = vpack(f, p);
-        else
-          for (int e = 0; e < left; ++e) p[e] = f[e];
+        if (left >= 8) {
+          st16(p, vpack(f, p));
+          st16(p + 4, vpack(f + 4, p));
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (e < left) p[e] = f[e];
+        }
       } else {
-        epilogue4(G.E, row, col, left, f);
+        epilogue16<8>(G.E, row, col, left, f);
       }
     }
   }
@@ -315,10 +402,13 @@ __global__ __launch_bounds__(256) void gemm16_join_kernel(const float* __restric
         for (int e = 0; e < 4; ++e) f[e] += __uint_as_float(v[e]);
       }
     } else {
-      for (int s = 0; s < splits; ++s)
-        for (int e = 0; e < left; ++e) f[e] += p[s * plane + e];
+      for (int s = 0; s < splits; ++s) {
+#pragma unroll
+        for (int e = 0; e < 3; ++e)
+          if (e < left) f[e] += p[s * plane + e];
+      }
     }
-    epilogue4(E, row, col, left, f);
+    epilogue16<4>(E, row, col, left, f);
   }
 }
 
@@ -383,7 +473,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void gemm16_few_kernel(Gemm16<T> G)
     for (int w = 0; w < FEW_WAVES; ++w)
 #pragma unroll
       for (int e = 0; e < 4; ++e) f[e] += red[w][row >> 4][row & 15][c + e];
-    epilogue4(G.E, row, c0 + c, left, f);
+    epilogue16<4>(G.E, row, c0 + c, left, f);
   }
 }
 
@@ -466,17 +556,18 @@ __global__ __launch_bounds__(256) void pad16_kernel(const unsigned short* __rest
 }
 
 // ---- geometry
-struct Plan16 { int bm, tiles_m, tiles_n, splits; };
+struct Plan16 { int bn, tiles_m, tiles_n, splits; };
 static Plan16 plan16(int M, int N, int K) {
   Plan16 p;
-  const int steps = (K + G16_BK - 1) / G16_BK;
-  const long long big = (long long)((M + 255) / 256) * ((N + 255) / 256);
-  p.bm = big >= 224 ? 256 : 128;
-  p.tiles_m = (M + p.bm - 1) / p.bm;
-  p.tiles_n = (N + p.bm - 1) / p.bm;
+  const int steps = (K + 63) / 64;
+  p.tiles_m = (M + 127) / 128;
+  const int force = env_int("HOPMI_G16_BN", 0);
+  p.bn = (long long)p.tiles_m * ((N + 255) / 256) >= 256 ? 256 : 128;
+  if (force) p.bn = force;
+  p.tiles_n = (N + p.bn - 1) / p.bn;
   const long long tiles = (long long)p.tiles_m * p.tiles_n;
   p.splits = 1;
-  if (p.bm == 128 && tiles < 256) {
+  if (p.bn == 128 && tiles < 256) {
     const long long want = 512 / tiles, most = steps / 4 > 0 ? steps / 4 : 1;
     p.splits = (int)(want < most ? want : most);
     if (p.splits < 1) p.splits = 1;
@@ -484,18 +575,12 @@ static Plan16 plan16(int M, int N, int K) {
   return p;
 }
 
-template <typename T, int BM, bool KA, bool KB> static void gemm16_go(const Gemm16<T>& G, hipStream_t st) {
-  constexpr int W = BM == 256 ? 8 : 4;
-  constexpr int bytes = 2 * 2 * BM * G16_BK * 2;
-  const unsigned grid = (unsigned)(G.tiles_m * G.tiles_n * G.splits);
-  if constexpr (BM == 256) {
-    static const hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void*>(gemm16_kernel<T, 256, 256, 2, 4, KA, KB>),
-                                                       hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    (void)once;
-    hipLaunchKernelGGL((gemm16_kernel<T, 256, 256, 2, 4, KA, KB>), dim3(grid), dim3(64 * W), bytes, st, G);
-  } else {
-    hipLaunchKernelGGL((gemm16_kernel<T, 128, 128, 2, 2, KA, KB>), dim3(grid), dim3(64 * W), bytes, st, G);
-  }
+template <typename T, int BM, int BN, int WR, int WC, int ST, int OCC, bool KA, bool KB> static void gemm16_go(const Gemm16<T>& G, hipStream_t st) {
+  constexpr int bytes = ST * (BM + BN) * G16_BK * 2;
+  const auto k = gemm16_kernel<T, BM, BN, WR, WC, ST, OCC, KA, KB>;
+  static const hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  (void)once;
+  hipLaunchKernelGGL(k, dim3((unsigned)(G.tiles_m * G.tiles_n * G.splits)), dim3(64 * WR * WC), bytes, st, G);
 }
 template <typename T> static void gemm16_run(Gemm16<T> G, int layout, float* ws, hipStream_t st) {
   if (layout == 0 && G.M <= FEW_ROWS) {
@@ -510,14 +595,14 @@ template <typename T> static void gemm16_run(Gemm16<T> G, int layout, float* ws,
   G.tiles_n = p.tiles_n;
   G.splits = p.splits;
   G.part = p.splits > 1 ? ws : nullptr;
-  if (p.bm == 256) {
-    if (layout == 0) gemm16_go<T, 256, true, true>(G, st);
-    else if (layout == 1) gemm16_go<T, 256, true, false>(G, st);
-    else gemm16_go<T, 256, false, false>(G, st);
+  if (p.bn == 256) {
+    if (layout == 0) gemm16_go<T, 128, 256, 2, 2, 3, 2, true, true>(G, st);
+    else if (layout == 1) gemm16_go<T, 128, 256, 2, 2, 3, 2, true, false>(G, st);
+    else gemm16_go<T, 128, 256, 2, 2, 3, 2, false, false>(G, st);
   } else {
-    if (layout == 0) gemm16_go<T, 128, true, true>(G, st);
-    else if (layout == 1) gemm16_go<T, 128, true, false>(G, st);
-    else gemm16_go<T, 128, false, false>(G, st);
+    if (layout == 0) gemm16_go<T, 128, 128, 2, 2, 3, 3, true, true>(G, st);
+    else if (layout == 1) gemm16_go<T, 128, 128, 2, 2, 3, 3, true, false>(G, st);
+    else gemm16_go<T, 128, 128, 2, 2, 3, 3, false, false>(G, st);
   }
   if (p.splits > 1) {
     const long long work = (long long)G.M * ((G.N + 3) / 4), blocks = (work + 255) / 256;
