@@ -12,8 +12,8 @@
 // v_mfma_f32_16x16x32: lane 16 q + n holds A[n][8 q ..], B[8 q ..][n] and D[4 q + r][n].  The result's COLUMNS are put on D's rows, so a
 // lane ends with four consecutive columns of one row and every epilogue access is 8 bytes.
 // LDS images are swizzled through the SOURCE address of each lane's 16 bytes (the DMA's LDS side is fixed: lane l at base + 16 l):
-//   contraction-contiguous tile [rows][64]: 128-byte rows, chunk c at c ^ ((row >> 1) & 7): 16 consecutive rows on 16 different slots
-//   result-contiguous tile [64][cols]: row k, 32-byte pair p at p ^ ((k & 3) | ((k >> 3) & 1) << 2): the eight rows that one half wave
+//   contraction-contiguous tile [rows][32]: swizzle() below
+//   result-contiguous tile [32][cols]: row k, 32-byte pair p at p ^ ((k & 3) | ((k >> 3) & 1) << 2): the eight rows that one half wave
 //   reads lie on eight different 32-byte groups
 // Edges: rows past the end are clamped to the last one (their results are not stored); contraction indices past the end read 16 bytes
 // of zeros instead, on both operands.  Operands whose rows do not start on 16 bytes, or end inside one, are copied once into rows
@@ -164,9 +164,10 @@ template <typename T> struct Gemm16 {
   int tiles_m, tiles_n, splits;
 };
 
-constexpr int G16_BK = 32;       // contraction per step: one MFMA's
+constexpr int G16_BK = 64;       // contraction per step, two MFMAs': rows of 128 bytes, whole lines, from every operand layout (with half of
+                                 // it the L2s' request rate was the bound: 64-byte requests, 80 % of the slots taken)
 
-// Staging of one operand's tile of R rows (KC: [R][32], else [32][R]) by NW waves, and its fragments.
+// Staging of one operand's tile of R rows (KC: [R][64], else [64][R]) by NW waves, and its fragments.
 template <typename T, int R, int NW, bool KC> struct Tile16 {
   static constexpr int BK = G16_BK, BYTES = R * BK * 2;
   static constexpr int NI = BYTES / 1024 / NW;     // 1 KiB DMA instructions per wave and step
@@ -184,7 +185,7 @@ template <typename T, int R, int NW, bool KC> struct Tile16 {
       const int row = (i * NW + wave) * (64 / LPR) + lane / LPR, s = lane % LPR;
       if (KC) {
         const int rc = min(row, r_total - 1 - r0);             // (r_total > r0)
-        off[i] = (unsigned)(rc * ld * 2 + (s ^ ((row >> 2) & 3)) * 16);
+        off[i] = (unsigned)(rc * ld * 2 + (s ^ ((row >> 1) & 7)) * 16);
       } else {
         const int c = ((((s >> 1) ^ ((row & 3) | ((row >> 3) & 1) << 2)) << 1) | (s & 1)) * 8;
         const int cc = min(c, ((r_total - r0 + 7) & ~7) - 8);  // (whole chunks: the operand's rows are padded to 8)
@@ -207,7 +208,7 @@ template <typename T, int R, int NW, bool KC> struct Tile16 {
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const int row = (i * NW + wave) * (64 / LPR) + lane / LPR;
-      const int k = KC ? ((lane % LPR) ^ ((row >> 2) & 3)) * 8 : row;
+      const int k = KC ? ((lane % LPR) ^ ((row >> 1) & 7)) * 8 : row;
       const char* src = k < left ? base + off[i] : reinterpret_cast<const char*>(g_zero16);
       __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
                                        (__attribute__((address_space(3))) void*)(lds + (i * NW + wave) * 1024), 16, 0, 0);
@@ -216,47 +217,47 @@ template <typename T, int R, int NW, bool KC> struct Tile16 {
   }
 };
 
-// fragments of NB 16-row blocks starting at block `b0` of a staged tile
+// fragments of NB 16-row blocks starting at block `b0` of a staged tile, contraction half h
 template <typename T, int R, int NB, bool KC>
-__device__ __forceinline__ void frags16(const char* lds, int b0, int n, int q, u32x4_t (&f)[NB]) {
+__device__ __forceinline__ void frags16(const char* lds, int b0, int h, int n, int q, u32x4_t (&f)[NB]) {
   if (KC) {
-    const char* p = lds + (b0 * 16 + n) * 64 + ((q ^ (n >> 2)) << 4);
+    const char* p = lds + (b0 * 16 + n) * 128 + (((h * 4 + q) ^ (n >> 1)) << 4);
 #pragma unroll
-    for (int j = 0; j < NB; ++j) f[j] = *reinterpret_cast<const u32x4_t*>(p + j * 1024);
+    for (int j = 0; j < NB; ++j) f[j] = *reinterpret_cast<const u32x4_t*>(p + j * 2048);
   } else {
     typedef short s4 __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) s4* s4p;
     const int sw = (n >> 2) | (q & 1) << 2;
-    const char* p = lds + (8 * q + (n >> 2)) * (R * 2) + (n & 3) * 8;
+    const char* p = lds + (h * 32 + 8 * q + (n >> 2)) * (R * 2) + (n & 3) * 8;
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
       const char* a = p + (((b0 + j) ^ sw) << 5);
       const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s4p)(a)), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s4p)(a + 4 * R * 2));
       typedef unsigned u2 __attribute__((ext_vector_type(2)));
-      const u2 l = __builtin_bit_cast(u2, lo), h = __builtin_bit_cast(u2, hi);
-      f[j] = u32x4_t{l[0], l[1], h[0], h[1]};
+      const u2 l = __builtin_bit_cast(u2, lo), h2 = __builtin_bit_cast(u2, hi);
+      f[j] = u32x4_t{l[0], l[1], h2[0], h2[1]};
     }
   }
 }
 
-// s_waitcnt vmcnt(N) lgkmcnt(0), as the builtin (the compiler's own counting then knows of it), and the barrier, with nothing moved across
-template <int N> __device__ __forceinline__ void wait_and_meet() {
-  static_assert(N < 64, "six bits");
-  __builtin_amdgcn_s_waitcnt((N & 15) | 7 << 4 | (N >> 4) << 14);
+// s_waitcnt vmcnt(0) lgkmcnt(0), as the builtin (the compiler's own counting then knows of it), and the barrier, with nothing moved across
+__device__ __forceinline__ void wait_and_meet() {
+  __builtin_amdgcn_s_waitcnt(7 << 4);
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
 
-// The steps are pipelined twice: ST LDS buffers of one step each, filled by DMA ST - 1 to ST steps ahead, and two sets of fragment
-// registers: a step's products run on fragments that were read during the step before, so neither the DMA nor the LDS reads are waited
-// for in a wave's own time.  One barrier per step.
-template <typename T, int BM, int BN, int WR, int WC, int ST, int OCC, bool KA, bool KB>
-__global__ __launch_bounds__(64 * WR * WC, OCC) void gemm16_kernel(Gemm16<T> G) {
+// Two LDS buffers of one step each, and two sets of fragment registers: the products of a step's half run on fragments that were read
+// during the half before, so neither the DMA (a whole step ahead) nor the LDS reads are waited for in a wave's own time.  One barrier per
+// step, between its halves: there, every wave has read all of this step (its buffer takes the step after the next) and the next step's
+// DMA has landed.
+template <typename T, int BM, int BN, int WR, int WC, bool KA, bool KB>
+__global__ __launch_bounds__(64 * WR * WC, 2) void gemm16_kernel(Gemm16<T> G) {
   constexpr int NW = WR * WC, RB = BM / WR / 16, CB = BN / WC / 16, BK = G16_BK;
   using TA = Tile16<T, BM, NW, KA>;
   using TB = Tile16<T, BN, NW, KB>;
-  constexpr int SB = TA::BYTES + TB::BYTES, NI = TA::NI + TB::NI;
+  constexpr int SB = TA::BYTES + TB::BYTES;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, q = lane >> 4;
   const int wr = wave / WC, wc = wave % WC;
@@ -297,11 +298,9 @@ __global__ __launch_bounds__(64 * WR * WC, OCC) void gemm16_kernel(Gemm16<T> G) 
     }
   };
   u32x4_t fa0[RB], fb0[CB], fa1[RB], fb1[CB];
-  char* cur = lds;
-  auto advance = [&] { cur = cur + SB == lds + ST * SB ? lds : cur + SB; };
-  auto fetch = [&](u32x4_t (&a)[RB], u32x4_t (&b)[CB]) {
-    frags16<T, BM, RB, KA>(cur, wr * RB, n, q, a);
-    frags16<T, BN, CB, KB>(cur + TA::BYTES, wc * CB, n, q, b);
+  auto fetch = [&](const char* from, int h, u32x4_t (&a)[RB], u32x4_t (&b)[CB]) {
+    frags16<T, BM, RB, KA>(from, wr * RB, h, n, q, a);
+    frags16<T, BN, CB, KB>(from + TA::BYTES, wc * CB, h, n, q, b);
   };
   auto multiply = [&](const u32x4_t (&a)[RB], const u32x4_t (&b)[CB]) {
 #pragma unroll
@@ -315,44 +314,35 @@ __global__ __launch_bounds__(64 * WR * WC, OCC) void gemm16_kernel(Gemm16<T> G) 
       __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
     }
   };
-#pragma unroll
-  for (int s = 0; s < ST; ++s)
-    if (s < steps) load_any(lds + s * SB, s);
-  if (steps >= ST) wait_and_meet<NI * (ST - 1)>();
-  else wait_and_meet<0>();
-  fetch(fa0, fb0);
-  // Step s: step s + 1 is in LDS once every wave's DMA for it is (counted, then the barrier); every wave has its fragments of step s, so
-  // that buffer takes step s + ST.
+  char *cur = lds, *nxt = lds + SB;
+  load_any(cur, 0);
+  wait_and_meet();
+  if (steps > 1) load_any(nxt, 1);
+  fetch(cur, 0, fa0, fb0);
   int s = 0;
-  for (; s + ST + 2 < steps; s += 2) {             // (steps that load whole ones)
-    wait_and_meet<NI * (ST - 2)>();
-    load(cur);
-    advance();
-    fetch(fa1, fb1);
+  for (; s + 3 < steps; ++s) {                     // (steps that load whole ones)
+    fetch(cur, 1, fa1, fb1);
     multiply(fa0, fb0);
-    wait_and_meet<NI * (ST - 2)>();
+    wait_and_meet();
     load(cur);
-    advance();
-    fetch(fa0, fb0);
+    fetch(nxt, 0, fa0, fb0);
     multiply(fa1, fb1);
+    char* t = cur; cur = nxt; nxt = t;
   }
 #pragma unroll 1
-  for (; s < steps; ++s) {                         // the last ST + 2 at most: the contraction's end may be among what they load
-    if (s + ST - 1 < steps) wait_and_meet<NI * (ST - 2)>();
-    else wait_and_meet<0>();
-    if (s + ST < steps) load_any(cur, s + ST);
-    advance();
-    fetch(fa1, fb1);                               // (past the last step: values that nothing uses)
+  for (; s < steps; ++s) {                         // the last three: the contraction's end may be in what they load
+    fetch(cur, 1, fa1, fb1);
     multiply(fa0, fb0);
-#pragma unroll
-    for (int i = 0; i < RB; ++i) fa0[i] = fa1[i];
-#pragma unroll
-    for (int j = 0; j < CB; ++j) fb0[j] = fb1[j];
+    wait_and_meet();
+    if (s + 2 < steps) load_any(cur, s + 2);
+    fetch(nxt, 0, fa0, fb0);                       // (past the last step: values that nothing uses)
+    multiply(fa1, fb1);
+    char* t = cur; cur = nxt; nxt = t;
   }
   // The results leave through LDS, 16 rows of every wave at a time: eight consecutive columns per lane then, whole lines per wave, and one
   // copy of the epilogue's code.  (The last reads of the buffers are awaited first; no DMA is in flight any more.)
   constexpr int LDC = BN + 4, VR = BN / 8, ROWS = WR * 16;
-  static_assert(ROWS * LDC * 4 <= ST * SB, "the staged rows fit the buffers");
+  static_assert(ROWS * LDC * 4 <= 2 * SB, "the staged rows fit the buffers");
   float* stage = reinterpret_cast<float*>(lds);
 #pragma unroll
   for (int i = 0; i < RB; ++i) {
@@ -560,10 +550,10 @@ struct Plan16 { int bn, tiles_m, tiles_n, splits; };
 static Plan16 plan16(int M, int N, int K) {
   Plan16 p;
   const int steps = (K + 63) / 64;
-  p.tiles_m = (M + 127) / 128;
   const int force = env_int("HOPMI_G16_BN", 0);
-  p.bn = (long long)p.tiles_m * ((N + 255) / 256) >= 256 ? 256 : 128;
+  p.bn = (long long)((M + 255) / 256) * ((N + 255) / 256) >= 224 ? 256 : 128;
   if (force) p.bn = force;
+  p.tiles_m = (M + p.bn - 1) / p.bn;
   p.tiles_n = (N + p.bn - 1) / p.bn;
   const long long tiles = (long long)p.tiles_m * p.tiles_n;
   p.splits = 1;
@@ -575,9 +565,9 @@ static Plan16 plan16(int M, int N, int K) {
   return p;
 }
 
-template <typename T, int BM, int BN, int WR, int WC, int ST, int OCC, bool KA, bool KB> static void gemm16_go(const Gemm16<T>& G, hipStream_t st) {
-  constexpr int bytes = ST * (BM + BN) * G16_BK * 2;
-  const auto k = gemm16_kernel<T, BM, BN, WR, WC, ST, OCC, KA, KB>;
+template <typename T, int BM, int BN, int WR, int WC, bool KA, bool KB> static void gemm16_go(const Gemm16<T>& G, hipStream_t st) {
+  constexpr int bytes = 2 * (BM + BN) * G16_BK * 2;
+  const auto k = gemm16_kernel<T, BM, BN, WR, WC, KA, KB>;
   static const hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
   (void)once;
   hipLaunchKernelGGL(k, dim3((unsigned)(G.tiles_m * G.tiles_n * G.splits)), dim3(64 * WR * WC), bytes, st, G);
@@ -596,13 +586,13 @@ template <typename T> static void gemm16_run(Gemm16<T> G, int layout, float* ws,
   G.splits = p.splits;
   G.part = p.splits > 1 ? ws : nullptr;
   if (p.bn == 256) {
-    if (layout == 0) gemm16_go<T, 128, 256, 2, 2, 3, 2, true, true>(G, st);
-    else if (layout == 1) gemm16_go<T, 128, 256, 2, 2, 3, 2, true, false>(G, st);
-    else gemm16_go<T, 128, 256, 2, 2, 3, 2, false, false>(G, st);
+    if (layout == 0) gemm16_go<T, 256, 256, 2, 4, true, true>(G, st);
+    else if (layout == 1) gemm16_go<T, 256, 256, 2, 4, true, false>(G, st);
+    else gemm16_go<T, 256, 256, 2, 4, false, false>(G, st);
   } else {
-    if (layout == 0) gemm16_go<T, 128, 128, 2, 2, 3, 3, true, true>(G, st);
-    else if (layout == 1) gemm16_go<T, 128, 128, 2, 2, 3, 3, true, false>(G, st);
-    else gemm16_go<T, 128, 128, 2, 2, 3, 3, false, false>(G, st);
+    if (layout == 0) gemm16_go<T, 128, 128, 2, 2, true, true>(G, st);
+    else if (layout == 1) gemm16_go<T, 128, 128, 2, 2, true, false>(G, st);
+    else gemm16_go<T, 128, 128, 2, 2, false, false>(G, st);
   }
   if (p.splits > 1) {
     const long long work = (long long)G.M * ((G.N + 3) / 4), blocks = (work + 255) / 256;
