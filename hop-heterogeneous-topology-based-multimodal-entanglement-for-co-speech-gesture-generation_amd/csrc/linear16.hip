@@ -12,13 +12,15 @@
 // v_mfma_f32_16x16x32: lane 16 q + n holds A[n][8 q ..], B[8 q ..][n] and D[4 q + r][n].  The result's COLUMNS are put on D's rows, so a
 // lane ends with four consecutive columns of one row and every epilogue access is 8 bytes.
 // LDS images are swizzled through the SOURCE address of each lane's 16 bytes (the DMA's LDS side is fixed: lane l at base + 16 l):
-//   contraction-contiguous tile [rows][32]: swizzle() below
-//   result-contiguous tile [32][cols]: row k, 32-byte pair p at p ^ ((k & 3) | ((k >> 3) & 1) << 2): the eight rows that one half wave
-//   reads lie on eight different 32-byte groups
+//   contraction-contiguous tile [rows][64]: 128-byte rows, 16-byte chunk c at c ^ ((row >> 1) & 7): the sixteen lanes that a 16-byte read serves
+//   together (0-3, 12-15, 20-23, 24-27, ...) lie on sixteen different slots
+//   result-contiguous tile [64][cols]: mn_swizzle() below: the eight rows that one half wave reads lie on eight different 32-byte groups
 // Edges: rows past the end are clamped to the last one (their results are not stored); contraction indices past the end read 16 bytes
 // of zeros instead, on both operands.  Operands whose rows do not start on 16 bytes, or end inside one, are copied once into rows
 // padded with zeros.
 #include "t16_dev.h"
+
+#include <type_traits>
 
 namespace hopmi {
 
@@ -38,7 +40,8 @@ __device__ __forceinline__ f32x4 mfma16x32(u32x4_t a, u32x4_t b, f32x4 c, const 
 // The normal distribution's tail, Phi(-u) for u >= 0, = exp(-u^2 / 2) Q(t) with t = 1 / (1 + p u): Q is e^{x^2} erfc(x) / 2 at x = u / sqrt 2,
 // a smooth function that a polynomial in t without constant term (Q -> 0 with t) meets to 5e-6 of its value on 0 <= u <= 14 (least
 // largest relative error, fitted against 64-bit values); beyond, exp(-u^2 / 2) is 0 in fp32.  RELATIVE accuracy far below the result's
-// rounding (2^-9 / 2^-12) also in the tail, at 11 instructions (erff takes several times that, in an epilogue that runs against MFMAs).
+// rounding (2^-9 / 2^-12) also in the tail.  The epilogue of a product with a short contraction is bound by these instructions (15 per
+// gelu, two of them at a quarter of the rate; erff alone takes twice that).
 __device__ __forceinline__ float gauss_tail(float u, float e) {      // e = exp(-u^2 / 2)
   const float t = __builtin_amdgcn_rcpf(fmaf(0.31f, u, 1.f));
   float q = fmaf(-0.07392919063568115f, t, 0.18044988811016083f);
@@ -46,34 +49,39 @@ __device__ __forceinline__ float gauss_tail(float u, float e) {      // e = exp(
   q = fmaf(q, t, 0.13342832028865814f);
   q = fmaf(q, t, 0.12044187635183334f);
   q = fmaf(q, t, 0.12386061996221542f);
-  return q * t * e;
+  return q * (t * e);
 }
-// silu is taken from h = exp(-|z| / 2): z h h keeps the negative tail where exp(z) itself would have left fp32's normal range.
-// Where a tail has underflowed the limits (z or 0) stand, at the infinities too; a NaN stays one.
+// With u = |z|: gelu(z) = max(z, 0) - u Phi(-u), silu(z) = max(z, 0) - u e^-u / (1 + e^-u), one expression for both signs, which keeps the
+// negative tails (e^-u as a square, whose root stays in fp32's normal range as far as u e^-u does).  u is bounded where the tail is 0, so
+// the limits z and 0 come out at the infinities too; max() drops a NaN, which is put back.
 __device__ __forceinline__ float act_fwd(float z, int act) {
-  if (act == ACT_RELU) return z > 0.f || z != z ? z : 0.f;
+  if (act == ACT_NONE) return z;
+  const float top = fmaxf(z, 0.f);
+  float y = top;
   if (act == ACT_GELU) {
-    const float tail = gauss_tail(fabsf(z), __expf(-0.5f * z * z));
-    return tail > 0.f || z != z ? (z > 0.f ? fmaf(-z, tail, z) : z * tail) : (z > 0.f ? z : -0.f);
+    const float u = fminf(fabsf(z), 14.f);
+    y = fmaf(-u, gauss_tail(u, __builtin_amdgcn_exp2f(u * u * -0.72134752044448170f)), top);
+  } else if (act == ACT_SILU) {
+    const float u = fminf(fabsf(z), 170.f), h = __builtin_amdgcn_exp2f(u * -0.72134752044448170f);
+    y = fmaf(-(u * h) * h, __builtin_amdgcn_rcpf(fmaf(h, h, 1.f)), top);
   }
-  if (act == ACT_SILU) {
-    const float h = __expf(-0.5f * fabsf(z)), d = __builtin_amdgcn_rcpf(fmaf(h, h, 1.f));
-    return z > 0.f ? z * d : (h > 0.f ? z * h * h * d : (z != z ? z : -0.f));
-  }
-  return z;
+  return z != z ? z : y;
 }
 __device__ __forceinline__ float act_grad(float z, int act) {
+  if (act == ACT_NONE) return 1.f;
   if (act == ACT_RELU) return z > 0.f ? 1.f : 0.f;
+  float g;
   if (act == ACT_GELU) {
-    const float e = __expf(-0.5f * z * z), tail = gauss_tail(fabsf(z), e);
-    return fmaf(e > 0.f || z != z ? z * 0.3989422804014327f : 0.f, e, z > 0.f ? 1.f - tail : tail);
+    const float u = fminf(fabsf(z), 14.f), e = __builtin_amdgcn_exp2f(u * u * -0.72134752044448170f), tail = gauss_tail(u, e);
+    const float d = fmaf(u * -0.3989422804014327f, e, tail);         // Phi(-u) - u phi(u)
+    g = z > 0.f ? 1.f - d : d;
+  } else {
+    const float u = fminf(fabsf(z), 170.f), h = __builtin_amdgcn_exp2f(u * -0.72134752044448170f), e = h * h;
+    const float r = __builtin_amdgcn_rcpf(1.f + e), s = e * r;       // the sigmoids of u and of -u
+    const float d = s * fmaf(-u, r, 1.f);
+    g = z > 0.f ? 1.f - d : d;
   }
-  if (act == ACT_SILU) {
-    const float h = __expf(-0.5f * fabsf(z)), e = h * h, d = __builtin_amdgcn_rcpf(1.f + e);
-    const float s = z > 0.f ? d : e * d, r = z > 0.f ? e * d : d;      // the sigmoid and what it lacks to 1
-    return e > 0.f || z != z ? s * fmaf(z, r, 1.f) : (z > 0.f ? 1.f : 0.f);
-  }
-  return 1.f;
+  return z != z ? z : g;
 }
 
 // V (4 or 8) consecutive elements at any element address
@@ -167,12 +175,18 @@ template <typename T> struct Gemm16 {
 constexpr int G16_BK = 64;       // contraction per step, two MFMAs': rows of 128 bytes, whole lines, from every operand layout (with half of
                                  // it the L2s' request rate was the bound: 64-byte requests, 80 % of the slots taken)
 
+// the 32-byte group of a result-contiguous tile's row k that holds its group 0 (group p: at p ^ this); rows of 128 bytes lie two to a line
+template <int R> __device__ __forceinline__ int mn_swizzle(int k) {
+  return R == 64 ? ((k >> 1) & 1) | ((k >> 3) & 1) << 1 : (k & 3) | ((k >> 3) & 1) << 2;
+}
+
 // Staging of one operand's tile of R rows (KC: [R][64], else [64][R]) by NW waves, and its fragments.
 template <typename T, int R, int NW, bool KC> struct Tile16 {
   static constexpr int BK = G16_BK, BYTES = R * BK * 2;
   static constexpr int NI = BYTES / 1024 / NW;     // 1 KiB DMA instructions per wave and step
   static constexpr int CPR = BK / 8;               // 16-byte chunks per row (KC)
   static constexpr int LPR = KC ? CPR : R / 8;     // lanes per tile row in memory order
+  static_assert(64 % LPR == 0 && NI * NW * 1024 == BYTES, "whole rows per instruction, whole instructions per wave");
   const char* base;                                // uniform; advances by one step
   long long adv;
   unsigned off[NI];                                // this lane's bytes from base
@@ -187,7 +201,7 @@ template <typename T, int R, int NW, bool KC> struct Tile16 {
         const int rc = min(row, r_total - 1 - r0);             // (r_total > r0)
         off[i] = (unsigned)(rc * ld * 2 + (s ^ ((row >> 1) & 7)) * 16);
       } else {
-        const int c = ((((s >> 1) ^ ((row & 3) | ((row >> 3) & 1) << 2)) << 1) | (s & 1)) * 8;
+        const int c = ((((s >> 1) ^ mn_swizzle<R>(row)) << 1) | (s & 1)) * 8;
         const int cc = min(c, ((r_total - r0 + 7) & ~7) - 8);  // (whole chunks: the operand's rows are padded to 8)
         off[i] = (unsigned)(row * ld * 2 + cc * 2);
       }
@@ -227,7 +241,7 @@ __device__ __forceinline__ void frags16(const char* lds, int b0, int h, int n, i
   } else {
     typedef short s4 __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) s4* s4p;
-    const int sw = (n >> 2) | (q & 1) << 2;
+    const int sw = mn_swizzle<R>(8 * q + (n >> 2));            // (the same for all the contraction indices this lane addresses)
     const char* p = lds + (h * 32 + 8 * q + (n >> 2)) * (R * 2) + (n & 3) * 8;
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
@@ -240,24 +254,25 @@ __device__ __forceinline__ void frags16(const char* lds, int b0, int h, int n, i
   }
 }
 
-// s_waitcnt vmcnt(0) lgkmcnt(0), as the builtin (the compiler's own counting then knows of it), and the barrier, with nothing moved across
-__device__ __forceinline__ void wait_and_meet() {
-  __builtin_amdgcn_s_waitcnt(7 << 4);
+// s_waitcnt vmcnt(N) lgkmcnt(0), as the builtin (the compiler's own counting then knows of it), and the barrier, with nothing moved across
+template <int N> __device__ __forceinline__ void wait_and_meet() {
+  static_assert(N < 64, "six bits");
+  __builtin_amdgcn_s_waitcnt((N & 15) | 7 << 4 | (N >> 4) << 14);
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
 
-// Two LDS buffers of one step each, and two sets of fragment registers: the products of a step's half run on fragments that were read
-// during the half before, so neither the DMA (a whole step ahead) nor the LDS reads are waited for in a wave's own time.  One barrier per
-// step, between its halves: there, every wave has read all of this step (its buffer takes the step after the next) and the next step's
-// DMA has landed.
-template <typename T, int BM, int BN, int WR, int WC, bool KA, bool KB>
+// ST LDS buffers of one step each, and two sets of fragment registers: the products of a step's half run on fragments that were read
+// during the half before, so neither the DMA (ST - 1 steps ahead) nor the LDS reads are waited for in a wave's own time.  One barrier per
+// step, between its halves: there, every wave has read all of this step (its buffer takes step s + ST) and step s + 1 has landed (the
+// younger DMA stays in flight: counted).
+template <typename T, int BM, int BN, int WR, int WC, int ST, bool KA, bool KB>
 __global__ __launch_bounds__(64 * WR * WC, 2) void gemm16_kernel(Gemm16<T> G) {
   constexpr int NW = WR * WC, RB = BM / WR / 16, CB = BN / WC / 16, BK = G16_BK;
   using TA = Tile16<T, BM, NW, KA>;
   using TB = Tile16<T, BN, NW, KB>;
-  constexpr int SB = TA::BYTES + TB::BYTES;
+  constexpr int SB = TA::BYTES + TB::BYTES, NI = TA::NI + TB::NI;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, q = lane >> 4;
   const int wr = wave / WC, wc = wave % WC;
@@ -315,60 +330,110 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void gemm16_kernel(Gemm16<T> G) {
     }
   };
   char *cur = lds, *nxt = lds + SB;
-  load_any(cur, 0);
-  wait_and_meet();
-  if (steps > 1) load_any(nxt, 1);
+  auto advance = [&] {
+    cur = nxt;
+    nxt = nxt + SB == lds + ST * SB ? lds : nxt + SB;
+  };
+#pragma unroll
+  for (int k = 0; k < ST; ++k)
+    if (k < steps) load_any(lds + k * SB, k);
+  if (steps >= ST) wait_and_meet<NI * (ST - 1)>();
+  else wait_and_meet<0>();
   fetch(cur, 0, fa0, fb0);
   int s = 0;
-  for (; s + 3 < steps; ++s) {                     // (steps that load whole ones)
+  for (; s + ST + 1 < steps; ++s) {                // (steps that load whole ones)
     fetch(cur, 1, fa1, fb1);
     multiply(fa0, fb0);
-    wait_and_meet();
+    wait_and_meet<NI * (ST - 2)>();
     load(cur);
     fetch(nxt, 0, fa0, fb0);
     multiply(fa1, fb1);
-    char* t = cur; cur = nxt; nxt = t;
+    advance();
   }
 #pragma unroll 1
-  for (; s < steps; ++s) {                         // the last three: the contraction's end may be in what they load
+  for (; s < steps; ++s) {                         // the last ST + 1: the contraction's end may be in what they load
     fetch(cur, 1, fa1, fb1);
     multiply(fa0, fb0);
-    wait_and_meet();
-    if (s + 2 < steps) load_any(cur, s + 2);
+    if (s + ST - 1 < steps) wait_and_meet<NI * (ST - 2)>();
+    else wait_and_meet<0>();
+    if (s + ST < steps) load_any(cur, s + ST);
     fetch(nxt, 0, fa0, fb0);                       // (past the last step: values that nothing uses)
     multiply(fa1, fb1);
-    char* t = cur; cur = nxt; nxt = t;
+    advance();
   }
-  // The results leave through LDS, 16 rows of every wave at a time: eight consecutive columns per lane then, whole lines per wave, and one
-  // copy of the epilogue's code.  (The last reads of the buffers are awaited first; no DMA is in flight any more.)
-  constexpr int LDC = BN + 4, VR = BN / 8, ROWS = WR * 16;
-  static_assert(ROWS * LDC * 4 <= 2 * SB, "the staged rows fit the buffers");
+  // The results leave through LDS, 16 rows of every wave at a time: a thread then has eight consecutive columns, the same ones in every
+  // row it meets (their bias is loaded once), a wave whole lines, and the epilogue's code is there twice, not once per register.  The
+  // residual of the next 16 rows travels meanwhile.  (The last reads of the buffers are awaited first; no DMA is in flight any more.)
+  constexpr int LDC = BN + 4, VR = BN / 8, ROWS = WR * 16, RPT = ROWS * VR / (64 * NW);
+  static_assert(ROWS * LDC * 4 <= ST * SB && (64 * NW) % VR == 0 && RPT * 64 * NW == ROWS * VR, "the staged rows fit the buffers and the threads");
   float* stage = reinterpret_cast<float*>(lds);
+  const Epi16<T>& E = G.E;
+  const int vc = threadIdx.x % VR * 8, col = c0 + vc, left = G.N - col;
+  auto row_of = [&](int i, int k) {
+    const int sr = threadIdx.x / VR + k * (64 * NW / VR);
+    return (long long)r0 + (sr / 16 * RB + i) * 16 + sr % 16;
+  };
+  const bool lean = left >= 8 && G.part == nullptr;
+  float b[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (lean && E.bias != nullptr) ldv(E.bias + col, b);
+  u32x4_t rn[RPT];
+  auto residual = [&](int i) {
 #pragma unroll
+    for (int k = 0; k < RPT; ++k) {
+      const long long row = row_of(i, k);
+      rn[k] = lean && E.res != nullptr && row < G.M ? ld16(E.res + row * E.ldr + col) : u32x4_t{0, 0, 0, 0};
+    }
+  };
+  residual(0);
+#pragma unroll 1
   for (int i = 0; i < RB; ++i) {
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < CB; ++j) *reinterpret_cast<f32x4*>(&stage[(wr * 16 + n) * LDC + (wc * CB + j) * 16 + 4 * q]) = acc[i][j];
+    for (int k = 0; k < RB; ++k)
+      if (k == i) {
+#pragma unroll
+        for (int j = 0; j < CB; ++j) *reinterpret_cast<f32x4*>(&stage[(wr * 16 + n) * LDC + (wc * CB + j) * 16 + 4 * q]) = acc[k][j];
+      }
+    u32x4_t rc[RPT];
+#pragma unroll
+    for (int k = 0; k < RPT; ++k) rc[k] = rn[k];
+    if (i + 1 < RB) residual(i + 1);
     __syncthreads();
-#pragma unroll 1
-    for (int v = threadIdx.x; v < ROWS * VR; v += 64 * NW) {
-      const int sr = v / VR, col = c0 + v % VR * 8, left = G.N - col;
-      const long long row = r0 + (sr / 16 * RB + i) * 16 + sr % 16;
+#pragma unroll
+    for (int k = 0; k < RPT; ++k) {
+      const long long row = row_of(i, k);
       if (row >= G.M || left <= 0) continue;
-      const f32x4 lo = *reinterpret_cast<const f32x4*>(&stage[sr * LDC + v % VR * 8]), hi = *reinterpret_cast<const f32x4*>(&stage[sr * LDC + v % VR * 8 + 4]);
+      const float* p = &stage[(threadIdx.x / VR + k * (64 * NW / VR)) * LDC + vc];
+      const f32x4 lo = *reinterpret_cast<const f32x4*>(p), hi = *reinterpret_cast<const f32x4*>(p + 4);
       float f[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-      if (G.part != nullptr) {
-        float* p = G.part + ((long long)split * G.M + row) * G.N + col;
+      if (lean) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] += b[e];
+        if (E.z != nullptr) stv(E.z + row * E.ldz + col, f);
+        if (E.act != ACT_NONE) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[e] = act_fwd(f[e], E.act);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] += vget(rc[k], e, G.A);
+        stv(E.C + row * E.ldc + col, f);
+      } else if (G.part != nullptr) {
+        float* o = G.part + ((long long)split * G.M + row) * G.N + col;
         if (left >= 8) {
-          st16(p, vpack(f, p));
-          st16(p + 4, vpack(f + 4, p));
+          st16(o, vpack(f, o));
+          st16(o + 4, vpack(f + 4, o));
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            if (e < left) p[e] = f[e];
+            if (e < left) o[e] = f[e];
         }
       } else {
-        epilogue16<8>(G.E, row, col, left, f);
+        for (int h = 0; h < 2; ++h) {              // (the result's last columns)
+          float g[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) g[e] = h ? f[4 + e] : f[e];
+          if (left > 4 * h) epilogue16<4>(E, row, col + 4 * h, left - 4 * h, g);
+        }
       }
     }
   }
@@ -546,28 +611,31 @@ __global__ __launch_bounds__(256) void pad16_kernel(const unsigned short* __rest
 }
 
 // ---- geometry
-struct Plan16 { int bn, tiles_m, tiles_n, splits; };
+struct Plan16 { int form, tiles_m, tiles_n, splits; };
 static Plan16 plan16(int M, int N, int K) {
   Plan16 p;
   const int steps = (K + 63) / 64;
   const int force = env_int("HOPMI_G16_BN", 0);
-  p.bn = (long long)((M + 255) / 256) * ((N + 255) / 256) >= 224 ? 256 : 128;
-  if (force) p.bn = force;
-  p.tiles_m = (M + p.bn - 1) / p.bn;
-  p.tiles_n = (N + p.bn - 1) / p.bn;
+  p.form = (long long)((M + 255) / 256) * ((N + 255) / 256) >= 224 ? 0 : 2;
+  if (force) p.form = force - 1;
+  const int bm = p.form == 0 ? 256 : p.form == 1 ? 192 : p.form == 4 ? 64 : 128, bn = p.form == 0 ? 256 : p.form == 4 ? 64 : 128;
+  p.tiles_m = (M + bm - 1) / bm;
+  p.tiles_n = (N + bn - 1) / bn;
   const long long tiles = (long long)p.tiles_m * p.tiles_n;
   p.splits = 1;
-  if (p.bn == 128 && tiles < 256) {
+  if (p.form == 2 && tiles < 256) {
     const long long want = 512 / tiles, most = steps / 4 > 0 ? steps / 4 : 1;
     p.splits = (int)(want < most ? want : most);
     if (p.splits < 1) p.splits = 1;
   }
+  const int fs = env_int("HOPMI_G16_SPLITS", 0);
+  if (fs) p.splits = fs < steps ? fs : steps;
   return p;
 }
 
-template <typename T, int BM, int BN, int WR, int WC, bool KA, bool KB> static void gemm16_go(const Gemm16<T>& G, hipStream_t st) {
-  constexpr int bytes = 2 * (BM + BN) * G16_BK * 2;
-  const auto k = gemm16_kernel<T, BM, BN, WR, WC, KA, KB>;
+template <typename T, int BM, int BN, int WR, int WC, int ST, bool KA, bool KB> static void gemm16_go(const Gemm16<T>& G, hipStream_t st) {
+  constexpr int bytes = ST * (BM + BN) * G16_BK * 2;
+  const auto k = gemm16_kernel<T, BM, BN, WR, WC, ST, KA, KB>;
   static const hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
   (void)once;
   hipLaunchKernelGGL(k, dim3((unsigned)(G.tiles_m * G.tiles_n * G.splits)), dim3(64 * WR * WC), bytes, st, G);
@@ -585,15 +653,18 @@ template <typename T> static void gemm16_run(Gemm16<T> G, int layout, float* ws,
   G.tiles_n = p.tiles_n;
   G.splits = p.splits;
   G.part = p.splits > 1 ? ws : nullptr;
-  if (p.bn == 256) {
-    if (layout == 0) gemm16_go<T, 256, 256, 2, 4, true, true>(G, st);
-    else if (layout == 1) gemm16_go<T, 256, 256, 2, 4, true, false>(G, st);
-    else gemm16_go<T, 256, 256, 2, 4, false, false>(G, st);
-  } else {
-    if (layout == 0) gemm16_go<T, 128, 128, 2, 2, true, true>(G, st);
-    else if (layout == 1) gemm16_go<T, 128, 128, 2, 2, true, false>(G, st);
-    else gemm16_go<T, 128, 128, 2, 2, false, false>(G, st);
-  }
+  auto go = [&](auto ka, auto kb) {
+    constexpr bool KA = decltype(ka)::value, KB = decltype(kb)::value;
+    if (p.form == 0) gemm16_go<T, 256, 256, 2, 4, 2, KA, KB>(G, st);
+    else if (p.form == 1) {
+      if constexpr (KA) gemm16_go<T, 192, 128, 2, 2, 2, KA, KB>(G, st);
+    } else if (p.form == 2) gemm16_go<T, 128, 128, 2, 2, 2, KA, KB>(G, st);
+    else if (p.form == 3) gemm16_go<T, 128, 128, 2, 2, 4, KA, KB>(G, st);
+    else gemm16_go<T, 64, 64, 2, 2, 4, KA, KB>(G, st);
+  };
+  if (layout == 0) go(std::true_type{}, std::true_type{});
+  else if (layout == 1) go(std::true_type{}, std::false_type{});
+  else go(std::false_type{}, std::false_type{});
   if (p.splits > 1) {
     const long long work = (long long)G.M * ((G.N + 3) / 4), blocks = (work + 255) / 256;
     hipLaunchKernelGGL((gemm16_join_kernel<T>), dim3((unsigned)(blocks < 2048 ? blocks : 2048)), dim3(256), 0, st, ws, p.splits, G.M, G.N, G.E);
