@@ -231,6 +231,13 @@ template <typename T, int R, int NW, bool KC> struct Tile16 {
   }
 };
 
+// The transposing LDS read: of the 16 lanes that share q, lane n addresses four elements of row n >> 2 and receives column n's four rows.
+// (restrict on the pointer is what tells the compiler's wait counting that the read does not touch what a DMA in flight writes: without
+// it every such read waited for ALL outstanding DMA, and the steps were not pipelined at all.)
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+__device__ __forceinline__ s16x4 read_transposed(lds_s16x4* __restrict__ p) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16(p); }
+
 // fragments of NB 16-row blocks starting at block `b0` of a staged tile, contraction half h
 template <typename T, int R, int NB, bool KC>
 __device__ __forceinline__ void frags16(const char* lds, int b0, int h, int n, int q, u32x4_t (&f)[NB]) {
@@ -239,14 +246,12 @@ __device__ __forceinline__ void frags16(const char* lds, int b0, int h, int n, i
 #pragma unroll
     for (int j = 0; j < NB; ++j) f[j] = *reinterpret_cast<const u32x4_t*>(p + j * 2048);
   } else {
-    typedef short s4 __attribute__((ext_vector_type(4)));
-    typedef __attribute__((address_space(3))) s4* s4p;
     const int sw = mn_swizzle<R>(8 * q + (n >> 2));            // (the same for all the contraction indices this lane addresses)
     const char* p = lds + (h * 32 + 8 * q + (n >> 2)) * (R * 2) + (n & 3) * 8;
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
       const char* a = p + (((b0 + j) ^ sw) << 5);
-      const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s4p)(a)), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s4p)(a + 4 * R * 2));
+      const s16x4 lo = read_transposed((lds_s16x4*)a), hi = read_transposed((lds_s16x4*)(a + 4 * R * 2));
       typedef unsigned u2 __attribute__((ext_vector_type(2)));
       const u2 l = __builtin_bit_cast(u2, lo), h2 = __builtin_bit_cast(u2, hi);
       f[j] = u32x4_t{l[0], l[1], h2[0], h2[1]};
@@ -611,26 +616,43 @@ __global__ __launch_bounds__(256) void pad16_kernel(const unsigned short* __rest
 }
 
 // ---- geometry
+// Five tile forms.  What a product costs is the rounds it takes to put its workgroups on the chip, the steps of each, and, where the
+// contraction is split, the join; no one form is best: 16384 x 4096 x 4096 takes 407 us in tiles of 256 x 256, 445 / 456 / 549 in 192 x 128 /
+// 128 x 128 (two buffers) / 128 x 128 (four); 4352 x 2304 x 768 27.0 / 23.8 / 27.2 / 31.9 and 30.7 in 64 x 64; 4352 x 768 x 2304 - / 32.4 / 27.2 /
+// 23.0 / 31.1; 512 x 768 x 768 - / 14.0 / 10.7 / 10.9 / 7.3.  So the choice is by a model of that cost, us, whose constants were fitted to
+// such times (24 products, all layouts, 1 to 16384 workgroups: within 15 % of nearly all of them):
+//   start     launch, first DMA, and the first tile's end
+//   alone     a step where a CU holds one workgroup;  together: where it holds as many as fit, for all of them
+//   end       a round's epilogue
+struct Form16 { int bm, bn, slots; float start, alone, together, end; };
+static constexpr Form16 FORMS16[] = {{256, 256, 256, 8.f, 1.55f, 1.55f, 1.f},     // 8 waves, 128 KB of LDS: one workgroup per CU
+                                     {192, 128, 512, 6.f, 0.69f, 1.35f, 1.5f},    // not for result-contiguous A (rows of 192)
+                                     {128, 128, 512, 4.5f, 0.62f, 0.89f, 2.5f},
+                                     {128, 128, 256, 5.f, 0.47f, 0.47f, 1.5f},    // four buffers: one workgroup per CU, DMA three steps ahead
+                                     {64, 64, 512, 3.f, 0.18f, 0.35f, 0.8f}};
 struct Plan16 { int form, tiles_m, tiles_n, splits; };
-static Plan16 plan16(int M, int N, int K) {
-  Plan16 p;
-  const int steps = (K + 63) / 64;
-  const int force = env_int("HOPMI_G16_BN", 0);
-  p.form = (long long)((M + 255) / 256) * ((N + 255) / 256) >= 224 ? 0 : 2;
-  if (force) p.form = force - 1;
-  const int bm = p.form == 0 ? 256 : p.form == 1 ? 192 : p.form == 4 ? 64 : 128, bn = p.form == 0 ? 256 : p.form == 4 ? 64 : 128;
-  p.tiles_m = (M + bm - 1) / bm;
-  p.tiles_n = (N + bn - 1) / bn;
-  const long long tiles = (long long)p.tiles_m * p.tiles_n;
-  p.splits = 1;
-  if (p.form == 2 && tiles < 256) {
-    const long long want = 512 / tiles, most = steps / 4 > 0 ? steps / 4 : 1;
-    p.splits = (int)(want < most ? want : most);
-    if (p.splits < 1) p.splits = 1;
+static Plan16 plan16(int M, int N, int K, int layout) {
+  const int steps = (K + G16_BK - 1) / G16_BK;
+  Plan16 best{0, 0, 0, 0};
+  float least = 0.f;
+  for (int f = 0; f < 5; ++f) {
+    if (f == 1 && layout == 2) continue;
+    const Form16& F = FORMS16[f];
+    const long long tm = ((long long)M + F.bm - 1) / F.bm, tn = ((long long)N + F.bn - 1) / F.bn, tiles = tm * tn;
+    // (more splits than fill the chip once, or steps of fewer than four, never pay: the join reads every partial result again)
+    for (int sp = 1; sp <= 32 && (sp == 1 || (tiles * sp <= F.slots && steps / sp >= 4)); sp += sp < 4 ? 1 : sp / 2) {
+      const long long wgs = tiles * sp, rounds = wgs / F.slots, rest = wgs - rounds * F.slots;
+      const float n = (float)((steps + sp - 1) / sp);
+      float t = F.start + (float)rounds * (n * F.together + F.end);
+      if (rest > 0) t += n * (rest > 256 ? F.together : F.alone) + F.end;
+      if (sp > 1) t += 4.f + 8.f * (float)sp * (float)M * (float)N / 12e6f;
+      if (best.splits == 0 || t < least) {
+        least = t;
+        best = Plan16{f, (int)tm, (int)tn, sp};
+      }
+    }
   }
-  const int fs = env_int("HOPMI_G16_SPLITS", 0);
-  if (fs) p.splits = fs < steps ? fs : steps;
-  return p;
+  return best;
 }
 
 template <typename T, int BM, int BN, int WR, int WC, int ST, bool KA, bool KB> static void gemm16_go(const Gemm16<T>& G, hipStream_t st) {
@@ -648,7 +670,7 @@ template <typename T> static void gemm16_run(Gemm16<T> G, int layout, float* ws,
     else hipLaunchKernelGGL((gemm16_few_kernel<T, 4>), grid, block, 0, st, G);
     return;
   }
-  const Plan16 p = plan16(G.M, G.N, G.K);
+  const Plan16 p = plan16(G.M, G.N, G.K, layout);
   G.tiles_m = p.tiles_m;
   G.tiles_n = p.tiles_n;
   G.splits = p.splits;
@@ -689,7 +711,7 @@ using namespace hopmi;
 extern "C" size_t hopmi_gemm16_ws_floats(int M, int N, int K, int layout) {
   if (M < 1 || N < 1 || K < 1 || layout < 0 || layout > 2) return 0;
   if (layout == 0 && M <= FEW_ROWS) return 0;
-  const Plan16 p = plan16(M, N, K);
+  const Plan16 p = plan16(M, N, K, layout);
   return p.splits > 1 ? (size_t)p.splits * M * N : 0;
 }
 
