@@ -6,39 +6,59 @@
 // write where something is written -- in place only if c < 1 (scaling by 1 changes nothing), into other tensors always.
 // Launch 1 (norm): the tensors are cut into chunks of 16 Ki elements, a workgroup takes chunks blockIdx, blockIdx + grid, ... and leaves
 // ONE sum; launch 2 (scale): every workgroup adds these <= 1024 sums in index order itself (8 KB out of the caches: less than a third
-// launch costs), forms c, and scales its chunks.  No atomics, nothing to clear, the same bits every time.
-// Sums are held in 64 bits: a value's square as one 64-bit fused step (the vector unit's 64-bit rate is far above what memory feeds it),
-// so neither the length of the list nor the size of a gradient (|g| up to 3.4e38 squares to 1e77) limits it.
-// The list travels in the kernel's arguments (up to GC_MAX tensors per launch, several launches for longer lists): no device table, no
-// copy, nothing that has to outlive the call, and a recording holds the addresses by itself.
+// launch costs), forms c, and scales its chunks, the list's last ones first.  No atomics, nothing to clear, the same bits every time.
+// Sums are held in 64 bits, so neither the length of the list nor the size of a gradient (|g| up to 3.4e38 squares to 1e77) limits it.
+// The list travels in the kernels' arguments (several launches for longer lists): no device table, no copy, nothing that has to outlive the
+// call, and a recording holds the addresses by itself.
 #include "t16_dev.h"
 
 namespace hopmi {
 
-constexpr int GC_MAX = 120;                        // tensors per launch: 120 x 28 bytes of kernel arguments
 constexpr int GC_CHUNK = 16384;                    // elements per work item: 256 threads x 16 vectors of 4, x 8 of 8
-constexpr int GC_GRID = 1024;                      // workgroups per launch at most = sums that the second launch adds
+constexpr int GC_GRID = 1024;                      // workgroups of the norm's launches at most = sums that the second launch adds
 
-struct GcList {
-  const void* in[GC_MAX];
-  void* out[GC_MAX];
-  long long n[GC_MAX];                             // elements
-  unsigned start[GC_MAX];                          // first chunk of the tensor; its type code in the top two bits
+// a list of tensors as kernel arguments, up to 4 KB of them: 250 tensors that are read (and written in place), 165 with outputs
+template <bool INTO> struct GcList {
+  static constexpr int MAX = INTO ? 165 : 250;
+  const void* in[MAX];
+  unsigned start[MAX];                             // first chunk of the tensor; its type code in the top two bits
+  unsigned tail[MAX];                              // elements in its last chunk
   int count;
   unsigned chunks;
+  void* out[INTO ? MAX : 1];
 };
+static_assert(sizeof(GcList<false>) <= 4040 && sizeof(GcList<true>) <= 4040, "kernel arguments of 4 KB");
 
 struct GcItem { int t; long long base; int cnt; int dt; };
-__device__ __forceinline__ GcItem gc_find(const GcList& L, unsigned chunk) {
+template <bool INTO> __device__ __forceinline__ GcItem gc_find(const GcList<INTO>& L, unsigned chunk) {
   int lo = 0, hi = L.count - 1;                    // the last tensor that starts at or before the chunk
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
     if ((L.start[mid] & 0x3fffffffu) <= chunk) lo = mid; else hi = mid - 1;
   }
-  const long long base = (long long)(chunk - (L.start[lo] & 0x3fffffffu)) * GC_CHUNK, left = L.n[lo] - base;
-  return GcItem{lo, base, left < GC_CHUNK ? (int)left : GC_CHUNK, (int)(L.start[lo] >> 30)};
+  const unsigned first = L.start[lo] & 0x3fffffffu, next = lo + 1 < L.count ? L.start[lo + 1] & 0x3fffffffu : L.chunks;
+  return GcItem{lo, (long long)(chunk - first) * GC_CHUNK, chunk + 1 == next ? (int)L.tail[lo] : GC_CHUNK, (int)(L.start[lo] >> 30)};
 }
 
+// The squares of a vector.  fp32: each in 64 bits.  16-bit values: a square is exact in fp32 and eight are added there first (eight 64-bit
+// conversions and steps per vector were what bound the kernel: 90 us for 160 M bf16 values, 57 us so) -- where that sum leaves fp32's
+// comfortable range, or is 0, they are taken again in 64 bits.
+template <typename T> __device__ __forceinline__ double gc_vec(const u32x4_t& v, const T* t) {
+  constexpr int V = Vec<T>::N;
+  if constexpr (V == 8) {
+    float f = 0.f;
+#pragma unroll
+    for (int e = 0; e < V; ++e) f = fmaf(vget(v, e, t), vget(v, e, t), f);
+    if (f > 0x1p-60f && f < 0x1p100f) return (double)f;
+  }
+  double s = 0.0;
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    const double d = (double)vget(v, e, t);
+    s = fma(d, d, s);
+  }
+  return s;
+}
 template <typename T> __device__ __forceinline__ double gc_squares(const T* p, int cnt) {
   constexpr int V = Vec<T>::N;
   double s = 0.0;
@@ -49,21 +69,9 @@ template <typename T> __device__ __forceinline__ double gc_squares(const T* p, i
 #pragma unroll
     for (int k = 0; k < 4; ++k) v[k] = ld16(p + (i + 256 * k) * V);
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const double d = (double)vget(v[k], e, p);
-        s = fma(d, d, s);
-      }
+    for (int k = 0; k < 4; ++k) s += gc_vec(v[k], p);
   }
-  for (; i < vecs; i += 256) {
-    const u32x4_t v = ld16(p + i * V);
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const double d = (double)vget(v, e, p);
-      s = fma(d, d, s);
-    }
-  }
+  for (; i < vecs; i += 256) s += gc_vec(ld16(p + i * V), p);
   if ((int)threadIdx.x < cnt - vecs * V) {
     const double d = (double)to_f(p[vecs * V + threadIdx.x]);
     s = fma(d, d, s);
@@ -79,7 +87,7 @@ __device__ __forceinline__ double block_sum256(double s, double* xch) {
   return xch[0] + xch[1] + xch[2] + xch[3];
 }
 
-__global__ __launch_bounds__(256) void gc_norm_kernel(GcList L, double* __restrict__ sums) {
+__global__ __launch_bounds__(256) void gc_norm_kernel(GcList<false> L, double* __restrict__ sums) {
   __shared__ double xch[4];
   double s = 0.0;
   for (unsigned c = blockIdx.x; c < L.chunks; c += gridDim.x) {
@@ -118,8 +126,9 @@ template <typename T, typename O> __device__ __forceinline__ void gc_scale(const
   }
 }
 
-__global__ __launch_bounds__(256) void gc_scale_kernel(GcList L, const double* __restrict__ sums, int nsums, float max_norm,
-                                                       float* __restrict__ norm_out, int in_place) {
+template <bool INTO>
+__global__ __launch_bounds__(256) void gc_scale_kernel(GcList<INTO> L, const double* __restrict__ sums, int nsums, float max_norm,
+                                                       float* __restrict__ norm_out) {
   __shared__ double xch[4];
   double s = 0.0;
   for (int i = threadIdx.x; i < nsums; i += 256) s += sums[i];
@@ -128,41 +137,47 @@ __global__ __launch_bounds__(256) void gc_scale_kernel(GcList L, const double* _
   const double q = (double)max_norm / (n + 1e-6);
   // (a NaN norm gives a NaN factor, an infinite one 0, as the formula says; without a limit the norm is all that is wanted)
   const float c = q > 1.0 || __builtin_isinf(max_norm) ? 1.f : (float)q;
-  if (in_place && c == 1.f) return;
+  if (!INTO && c == 1.f) return;
   for (unsigned k = blockIdx.x; k < L.chunks; k += gridDim.x) {
-    const GcItem it = gc_find(L, k);
-    if (it.dt == T_F32) {
-      const float* p = static_cast<const float*>(L.in[it.t]) + it.base;
-      gc_scale(p, static_cast<float*>(L.out[it.t]) + it.base, it.cnt, c);
-    } else if (it.dt == T_BF16) {
-      const __bf16* p = static_cast<const __bf16*>(L.in[it.t]) + it.base;
-      if (in_place) gc_scale(p, static_cast<__bf16*>(L.out[it.t]) + it.base, it.cnt, c);
-      else gc_scale(p, static_cast<float*>(L.out[it.t]) + it.base, it.cnt, c);
-    } else {
-      const _Float16* p = static_cast<const _Float16*>(L.in[it.t]) + it.base;
-      if (in_place) gc_scale(p, static_cast<_Float16*>(L.out[it.t]) + it.base, it.cnt, c);
-      else gc_scale(p, static_cast<float*>(L.out[it.t]) + it.base, it.cnt, c);
-    }
+    const GcItem it = gc_find(L, L.chunks - 1 - k);              // from the end: what the norm read last is still in the caches
+    auto scale = [&](auto type) {
+      using T = decltype(type);
+      const T* p = static_cast<const T*>(L.in[it.t]) + it.base;
+      if constexpr (INTO) gc_scale(p, static_cast<float*>(L.out[it.t]) + it.base, it.cnt, c);
+      else gc_scale(p, const_cast<T*>(p), it.cnt, c);
+    };
+    if (it.dt == T_F32) scale(float{});
+    else if (it.dt == T_BF16) scale(__bf16{});
+    else scale(_Float16{});
   }
 }
 
 // fills L with tensors [first, ...) of the list; returns the next one.  Empty tensors take no place.
-static int gc_fill(GcList& L, const void* const* in, void* const* out, const long long* n, const int* dtypes, int count, int first) {
+struct GcArgs { const void* const* in; void* const* out; const long long* n; const int* dtypes; int count; };
+template <bool INTO> static int gc_fill(GcList<INTO>& L, const GcArgs& A, int first) {
   L.count = 0;
   L.chunks = 0;
   int t = first;
-  for (; t < count && L.count < GC_MAX; ++t) {
-    if (n[t] == 0) continue;
-    const long long c = (n[t] + GC_CHUNK - 1) / GC_CHUNK;
+  for (; t < A.count && L.count < GcList<INTO>::MAX; ++t) {
+    if (A.n[t] == 0) continue;
+    const long long c = (A.n[t] + GC_CHUNK - 1) / GC_CHUNK;
     if (L.chunks + c > 0x3fffffffLL) break;
-    L.in[L.count] = in[t];
-    L.out[L.count] = out != nullptr ? out[t] : const_cast<void*>(in[t]);
-    L.n[L.count] = n[t];
-    L.start[L.count] = L.chunks | ((unsigned)dtypes[t] << 30);
+    L.in[L.count] = A.in[t];
+    if (INTO) L.out[L.count] = A.out[t];
+    L.start[L.count] = L.chunks | ((unsigned)A.dtypes[t] << 30);
+    L.tail[L.count] = (unsigned)(A.n[t] - (c - 1) * GC_CHUNK);
     ++L.count;
     L.chunks += (unsigned)c;
   }
   return t;
+}
+template <bool INTO> static void gc_scale_all(const GcArgs& A, const double* sums, int nsums, float max_norm, float* norm, hipStream_t st) {
+  GcList<INTO> L;
+  for (int k = 0, t = 0; k == 0 || t < A.count; ++k) {                         // (no values at all: the norm, 0, and nothing to scale)
+    t = gc_fill(L, A, t);
+    const unsigned g = L.chunks < 2048u ? (L.chunks > 0 ? L.chunks : 1u) : 2048u;
+    hipLaunchKernelGGL((gc_scale_kernel<INTO>), dim3(g), dim3(256), 0, st, L, sums, nsums, max_norm, k == 0 ? norm : nullptr);
+  }
 }
 
 }  // namespace hopmi
@@ -184,10 +199,11 @@ extern "C" int hopmi_grad_clip(const void* const* grads, void* const* outs, cons
       set_error("hopmi_grad_clip: tensor %d: n=%lld dtype=%d, or a null pointer", t, numels[t], dtypes[t]);
       return HOPMI_EINVAL;
     }
-  GcList L;
+  const GcArgs A{grads, outs, numels, dtypes, count};
+  GcList<false> L;
   int lists = 0;
   for (int t = 0; t < count; ++lists) {
-    t = gc_fill(L, grads, outs, numels, dtypes, count, t);
+    t = gc_fill(L, A, t);
     if (L.count == 0) break;
   }
   // every launch of the norm gets its share of the sums' places
@@ -196,15 +212,12 @@ extern "C" int hopmi_grad_clip(const void* const* grads, void* const* outs, cons
   double* sums = static_cast<double*>(ws);
   int nsums = 0;
   for (int k = 0, t = 0; k < lists; ++k) {
-    t = gc_fill(L, grads, outs, numels, dtypes, count, t);
+    t = gc_fill(L, A, t);
     const int cap = GC_GRID / lists, g = L.chunks < (unsigned)cap ? (int)L.chunks : cap;
     hipLaunchKernelGGL(gc_norm_kernel, dim3(g), dim3(256), 0, st, L, sums + nsums);
     nsums += g;
   }
-  for (int k = 0, t = 0; k < (lists > 0 ? lists : 1); ++k) {                   // (no values at all: the norm, 0, and nothing to scale)
-    t = gc_fill(L, grads, outs, numels, dtypes, count, t);
-    const unsigned g = L.chunks < 2048u ? (L.chunks > 0 ? L.chunks : 1u) : 2048u;
-    hipLaunchKernelGGL(gc_scale_kernel, dim3(g), dim3(256), 0, st, L, sums, nsums, max_norm, k == 0 ? norm : nullptr, outs == nullptr);
-  }
+  if (outs != nullptr) gc_scale_all<true>(A, sums, nsums, max_norm, norm, st);
+  else gc_scale_all<false>(A, sums, nsums, max_norm, norm, st);
   return check_launch("hopmi_grad_clip");
 }

@@ -4,7 +4,7 @@
 //   dx = r (g dy - mean_d(g dy) - xh mean_d(g dy xh))       dg = sum_rows dy xh       db = sum_rows dy
 //
 // Bound: HBM (8 / 22 operations per element against 4-8 / 6-12 bytes).  So each pass reads x (and dy) once: a row stays in the
-// registers of one wave (up to 256 16-byte vectors), of a 256-thread workgroup (up to 1024) or of a 1024-thread one (up to 2048);
+// registers of one wave (up to 256 16-byte vectors) or of a workgroup of 256 (up to 512), 512 (1024) or 1024 threads (2048);
 // wider rows are re-read (from the caches) by the looped form.  The variance is taken around the mean, not as E x^2 - mu^2: the row
 // is in registers, a second pass over it costs no memory.
 // The weights' gradients are sums over the rows: a workgroup walks rows blockIdx, blockIdx + grid, ... and keeps its columns' sums in
@@ -350,10 +350,10 @@ __global__ __launch_bounds__(1024) void ln_reduce_kernel(const float* __restrict
   }
 }
 
-// which form a row width takes, by its number of 16-byte vectors: a wave up to 256, 256 threads up to 1024, 1024 threads up to 2048
+// which form a row width takes, by its number of 16-byte vectors: a wave up to 256, then two vectors per thread
 static int ln_form(int D, int dtype) {
   const int vecs = D / (dtype == T_F32 ? 4 : 8);
-  return vecs <= 256 ? 64 : vecs <= 1024 ? 256 : vecs <= 2048 ? 1024 : 0;
+  return vecs <= 256 ? 64 : vecs <= 512 ? 256 : vecs <= 1024 ? 512 : vecs <= 2048 ? 1024 : 0;
 }
 // workgroups of a backward launch: rows in whole passes over an even grid of at most 512 workgroups
 static int ln_bwd_grid(int M, int form) {
@@ -367,7 +367,7 @@ template <typename T, typename WT, int NV, int TPR>
 static void ln_fwd_go(const void* x, long long ldx, const void* w, const void* b, void* y, float* mean, float* rstd, int M, int D,
                       float eps, hipStream_t st) {
   const long long units = TPR == 64 ? ((long long)M + 3) / 4 : M;
-  const int cap = TPR == 64 ? 2048 : TPR == 256 ? 1536 : 512;
+  const int cap = TPR == 64 ? 2048 : TPR == 256 ? 1536 : TPR == 512 ? 1024 : 512;
   hipLaunchKernelGGL((ln_fwd_kernel<T, WT, NV, TPR>), dim3((unsigned)(units < cap ? units : cap)), dim3(TPR == 64 ? 256 : TPR), 0, st,
                      static_cast<const T*>(x), ldx, static_cast<const WT*>(w), static_cast<const WT*>(b), static_cast<T*>(y), mean, rstd, M, D, eps);
 }
@@ -379,8 +379,8 @@ static void ln_fwd_typed(const void* x, long long ldx, const void* w, const void
   if (form == 64 && vecs <= 64) ln_fwd_go<T, WT, 1, 64>(x, ldx, w, b, y, mean, rstd, M, D, eps, st);
   else if (form == 64 && vecs <= 128) ln_fwd_go<T, WT, 2, 64>(x, ldx, w, b, y, mean, rstd, M, D, eps, st);
   else if (form == 64) ln_fwd_go<T, WT, 4, 64>(x, ldx, w, b, y, mean, rstd, M, D, eps, st);
-  else if (form == 256 && vecs <= 512) ln_fwd_go<T, WT, 2, 256>(x, ldx, w, b, y, mean, rstd, M, D, eps, st);
-  else if (form == 256) ln_fwd_go<T, WT, 4, 256>(x, ldx, w, b, y, mean, rstd, M, D, eps, st);
+  else if (form == 256) ln_fwd_go<T, WT, 2, 256>(x, ldx, w, b, y, mean, rstd, M, D, eps, st);
+  else if (form == 512) ln_fwd_go<T, WT, 2, 512>(x, ldx, w, b, y, mean, rstd, M, D, eps, st);
   else if (form == 1024) ln_fwd_go<T, WT, 2, 1024>(x, ldx, w, b, y, mean, rstd, M, D, eps, st);
   else
     hipLaunchKernelGGL((ln_fwd_loop_kernel<T, WT>), dim3(M < 512 ? M : 512), dim3(1024), 0, st, static_cast<const T*>(x), ldx, static_cast<const WT*>(w), static_cast<const WT*>(b),
@@ -402,8 +402,8 @@ static void ln_bwd_typed(const void* x, long long ldx, const void* dy, const flo
   if (form == 64 && vecs <= 64) ln_bwd_go<T, WT, 1, 64>(x, ldx, dy, mean, rstd, w, dx, part, M, D, st);
   else if (form == 64 && vecs <= 128) ln_bwd_go<T, WT, 2, 64>(x, ldx, dy, mean, rstd, w, dx, part, M, D, st);
   else if (form == 64) ln_bwd_go<T, WT, 4, 64>(x, ldx, dy, mean, rstd, w, dx, part, M, D, st);
-  else if (form == 256 && vecs <= 512) ln_bwd_go<T, WT, 2, 256>(x, ldx, dy, mean, rstd, w, dx, part, M, D, st);
-  else if (form == 256) ln_bwd_go<T, WT, 4, 256>(x, ldx, dy, mean, rstd, w, dx, part, M, D, st);
+  else if (form == 256) ln_bwd_go<T, WT, 2, 256>(x, ldx, dy, mean, rstd, w, dx, part, M, D, st);
+  else if (form == 512) ln_bwd_go<T, WT, 2, 512>(x, ldx, dy, mean, rstd, w, dx, part, M, D, st);
   else if (form == 1024) ln_bwd_go<T, WT, 2, 1024>(x, ldx, dy, mean, rstd, w, dx, part, M, D, st);
   else {
     if (dx != nullptr)

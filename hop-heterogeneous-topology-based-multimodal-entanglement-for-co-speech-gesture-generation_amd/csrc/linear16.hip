@@ -53,35 +53,34 @@ __device__ __forceinline__ float gauss_tail(float u, float e) {      // e = exp(
 }
 // With u = |z|: gelu(z) = max(z, 0) - u Phi(-u), silu(z) = max(z, 0) - u e^-u / (1 + e^-u), one expression for both signs, which keeps the
 // negative tails (e^-u as a square, whose root stays in fp32's normal range as far as u e^-u does).  u is bounded where the tail is 0, so
-// the limits z and 0 come out at the infinities too; max() drops a NaN, which is put back.
+// the limits z and 0 come out at the infinities too; minimum and maximum are the forms that pass a NaN on.
+__device__ __forceinline__ float bounded(float z, float most) { return __builtin_elementwise_minimum(fabsf(z), most); }
 __device__ __forceinline__ float act_fwd(float z, int act) {
   if (act == ACT_NONE) return z;
-  const float top = fmaxf(z, 0.f);
-  float y = top;
+  const float top = __builtin_elementwise_maximum(z, 0.f);
   if (act == ACT_GELU) {
-    const float u = fminf(fabsf(z), 14.f);
-    y = fmaf(-u, gauss_tail(u, __builtin_amdgcn_exp2f(u * u * -0.72134752044448170f)), top);
-  } else if (act == ACT_SILU) {
-    const float u = fminf(fabsf(z), 170.f), h = __builtin_amdgcn_exp2f(u * -0.72134752044448170f);
-    y = fmaf(-(u * h) * h, __builtin_amdgcn_rcpf(fmaf(h, h, 1.f)), top);
+    const float u = bounded(z, 14.f);
+    return fmaf(-u, gauss_tail(u, __builtin_amdgcn_exp2f(u * u * -0.72134752044448170f)), top);
   }
-  return z != z ? z : y;
+  if (act == ACT_SILU) {
+    const float u = bounded(z, 170.f), h = __builtin_amdgcn_exp2f(u * -0.72134752044448170f);
+    return fmaf(-(u * h) * h, __builtin_amdgcn_rcpf(fmaf(h, h, 1.f)), top);
+  }
+  return top;
 }
 __device__ __forceinline__ float act_grad(float z, int act) {
   if (act == ACT_NONE) return 1.f;
   if (act == ACT_RELU) return z > 0.f ? 1.f : 0.f;
-  float g;
+  float d;                                         // act'(-u); act'(u) = 1 - act'(-u)
   if (act == ACT_GELU) {
-    const float u = fminf(fabsf(z), 14.f), e = __builtin_amdgcn_exp2f(u * u * -0.72134752044448170f), tail = gauss_tail(u, e);
-    const float d = fmaf(u * -0.3989422804014327f, e, tail);         // Phi(-u) - u phi(u)
-    g = z > 0.f ? 1.f - d : d;
+    const float u = bounded(z, 14.f), e = __builtin_amdgcn_exp2f(u * u * -0.72134752044448170f);
+    d = fmaf(u * -0.3989422804014327f, e, gauss_tail(u, e));         // Phi(-u) - u phi(u)
   } else {
-    const float u = fminf(fabsf(z), 170.f), h = __builtin_amdgcn_exp2f(u * -0.72134752044448170f), e = h * h;
+    const float u = bounded(z, 170.f), h = __builtin_amdgcn_exp2f(u * -0.72134752044448170f), e = h * h;
     const float r = __builtin_amdgcn_rcpf(1.f + e), s = e * r;       // the sigmoids of u and of -u
-    const float d = s * fmaf(-u, r, 1.f);
-    g = z > 0.f ? 1.f - d : d;
+    d = s * fmaf(-u, r, 1.f);
   }
-  return z != z ? z : g;
+  return z > 0.f ? 1.f - d : d;
 }
 
 // V (4 or 8) consecutive elements at any element address
@@ -545,24 +544,46 @@ __global__ __launch_bounds__(256) void act_bwd16_kernel(const T* __restrict__ dy
   __shared__ float red[3][512];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = blockIdx.x * 512 + lane * 8, left = N - col;
   float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (left > 0)
-    for (long long row = (long long)blockIdx.y * 4 + wave; row < M; row += (long long)gridDim.y * 4) {
-      float g[8], v[8];
-      const T* p = dy + row * ldy + col;
-      if (left >= 8) ldf<8>(p, g);
-      else {
+  const long long first = (long long)blockIdx.y * 4 + wave, step = (long long)gridDim.y * 4;
+  auto finish = [&](long long row, float (&g)[8], const u32x4_t& zv) {
+    if (act != ACT_NONE) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) g[e] = e < left ? to_f(p[e]) : 0.f;
-      }
-      if (act != ACT_NONE) {
-        ldf<8>(z + row * ldz + col, v);              // (rows of z are padded to 8)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) g[e] = e < left ? g[e] * act_grad(v[e], act) : 0.f;
-      }
-      if (dz != nullptr) st16(dz + row * ldd + col, vpack(g, p));
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s[e] += g[e];
+      for (int e = 0; e < 8; ++e) g[e] *= act_grad(vget(zv, e, dy), act);
     }
+    if (dz != nullptr) st16(dz + row * ldd + col, vpack(g, dy));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s[e] += g[e];
+  };
+  if (left >= 8) {
+    for (long long row = first; row < M; row += 2 * step) {      // two rows' loads in flight
+      u32x4_t gv[2], zv[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        if (row + k * step < M) {
+          gv[k] = ld16(dy + (row + k * step) * ldy + col);
+          if (act != ACT_NONE) zv[k] = ld16(z + (row + k * step) * ldz + col);
+        }
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        if (row + k * step < M) {
+          float g[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) g[e] = vget(gv[k], e, dy);
+          finish(row + k * step, g, zv[k]);
+        }
+    }
+  } else if (left > 0) {                                         // the rows' ends (those of z and dz are padded to 8)
+    for (long long row = first; row < M; row += step) {
+      float g[8];
+      const T* p = dy + row * ldy + col;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) g[e] = e < left ? to_f(p[e]) : 0.f;
+      u32x4_t zv = act != ACT_NONE ? ld16(z + row * ldz + col) : u32x4_t{0, 0, 0, 0};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) zv[w] &= (2 * w < left ? 0xffffu : 0u) | (2 * w + 1 < left ? 0xffff0000u : 0u);   // (z's padding holds anything)
+      finish(row, g, zv);
+    }
+  }
   if (part == nullptr) return;
   if (wave > 0) {
 #pragma unroll

@@ -60,10 +60,20 @@ template <int N, typename T> __device__ __forceinline__ void ldf(const T* p, flo
   }
 }
 
+// The sum over a wave's 64 lanes, in every lane, without the LDS pipe: lane exchanges within 16 lanes (DPP), then between the 16-lane rows
+// and the halves (gfx950's row swaps).  Each exchange adds two values that both partners hold, so all lanes end with the same bits.
+template <int CTRL> __device__ __forceinline__ float dpp_add(float v) {
+  return v + __uint_as_float((unsigned)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL, 0xf, 0xf, true));
+}
 __device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-  return v;
+  v = dpp_add<0xb1>(v);                            // lanes 1, 0, 3, 2
+  v = dpp_add<0x4e>(v);                            // 2, 3, 0, 1
+  v = dpp_add<0x141>(v);                           // mirrored within 8
+  v = dpp_add<0x140>(v);                           // mirrored within 16
+  const auto h = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(h[0]) + __uint_as_float(h[1]);
+  const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(w[0]) + __uint_as_float(w[1]);
 }
 
 }  // namespace hopmi

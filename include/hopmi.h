@@ -584,7 +584,7 @@ int hopmi_act_bwd16(const void* dy, long long ldy, const void* z, long long ldz,
 /* Global gradient norm and clipping: *norm (device, fp32) = the 2-norm over all `count` tensors, c = min(1, max_norm / (*norm + 1e-6)),
  * and outs[t] = c grads[t]: outs NULL scales in place (nothing is written when c = 1), otherwise outs[t] is an fp32 tensor of the same
  * numel.  grads / outs / numels / dtypes are HOST arrays, read before the call returns (the list travels in the kernels' arguments);
- * at most 15 360 non-empty tensors.  Sums in 64 bits, in a fixed order.  A NaN or infinite norm scales by NaN or 0, as the formula
+ * at most 32 000 non-empty tensors.  Sums in 64 bits, in a fixed order.  A NaN or infinite norm scales by NaN or 0, as the formula
  * says.  ws: hopmi_grad_clip_ws_bytes() bytes on 8. */
 size_t hopmi_grad_clip_ws_bytes(void);
 int hopmi_grad_clip(const void* const* grads, void* const* outs, const long long* numels, const int* dtypes, int count, float max_norm,

@@ -86,6 +86,6 @@ def test_grad_clip_entry_point_refuses():
     for bn, bdt, bp in ((-1, 0, 16), (4, 3, 16), (4, 0, None)):
         assert L.hopmi_grad_clip((ctypes.c_void_p * 1)(bp), None, (ctypes.c_longlong * 1)(bn), (ctypes.c_int * 1)(bdt), 1, 1.0, ONE, ONE, None) == -1
         assert "tensor 0" in _last()
-    many = 120 * 129
+    many = 250 * 129
     assert L.hopmi_grad_clip((ctypes.c_void_p * many)(*[16] * many), None, (ctypes.c_longlong * many)(*[1] * many),
                              (ctypes.c_int * many)(), many, 1.0, ONE, ONE, None) == -1 and "more than one call" in _last()

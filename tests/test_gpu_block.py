@@ -404,7 +404,7 @@ def _clip_case(seed, count, dtypes, scale=1.0, odd=True):
 
 
 @pytest.mark.parametrize("dtypes", [["fp32"], ["bf16"], ["fp16"], ["fp32", "bf16", "fp16"]])
-@pytest.mark.parametrize("count", [1, 7, 119, 120, 121, 300])
+@pytest.mark.parametrize("count", [1, 7, 119, 120, 121, 164, 165, 166, 250, 251, 300])
 @pytest.mark.parametrize("into", [False, True])
 def test_grad_clip_norm_and_values(count, dtypes, into):
     for limit in (0.5, 1e6, 0.0):
