@@ -206,16 +206,14 @@ template <typename T, int R, int NW, bool KC> struct Tile16 {
       }
     }
   }
-  // issues a whole step's DMA into `lds`
-  __device__ __forceinline__ void load(char* lds, int wave) {
+  // instruction i of a whole step's DMA into `lds`; advance() after the last
+  __device__ __forceinline__ void issue(char* lds, int wave, int i) const {
 #ifdef __HIP_DEVICE_COMPILE__                      // (the host pass has no such type)
     const __amdgpu_buffer_rsrc_t src = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, -1, 0x00020000);
-#pragma unroll
-    for (int i = 0; i < NI; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (__attribute__((address_space(3))) void*)(lds + (i * NW + wave) * 1024), 16, off[i], 0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (__attribute__((address_space(3))) void*)(lds + (i * NW + wave) * 1024), 16, off[i], 0, 0, 0);
 #endif
-    base += adv;
   }
+  __device__ __forceinline__ void advance() { base += adv; }
   // ... of a step of which only `left` contraction indices exist (KC: rounded up to 8); zeros behind them
   __device__ __forceinline__ void load_edge(char* lds, int left, int lane, int wave) {
 #pragma unroll
@@ -237,25 +235,16 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 __device__ __forceinline__ s16x4 read_transposed(lds_s16x4* __restrict__ p) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16(p); }
 
-// fragments of NB 16-row blocks starting at block `b0` of a staged tile, contraction half h
-template <typename T, int R, int NB, bool KC>
-__device__ __forceinline__ void frags16(const char* lds, int b0, int h, int n, int q, u32x4_t (&f)[NB]) {
-  if (KC) {
-    const char* p = lds + (b0 * 16 + n) * 128 + (((h * 4 + q) ^ (n >> 1)) << 4);
-#pragma unroll
-    for (int j = 0; j < NB; ++j) f[j] = *reinterpret_cast<const u32x4_t*>(p + j * 2048);
-  } else {
-    const int sw = mn_swizzle<R>(8 * q + (n >> 2));            // (the same for all the contraction indices this lane addresses)
-    const char* p = lds + (h * 32 + 8 * q + (n >> 2)) * (R * 2) + (n & 3) * 8;
-#pragma unroll
-    for (int j = 0; j < NB; ++j) {
-      const char* a = p + (((b0 + j) ^ sw) << 5);
-      const s16x4 lo = read_transposed((lds_s16x4*)a), hi = read_transposed((lds_s16x4*)(a + 4 * R * 2));
-      typedef unsigned u2 __attribute__((ext_vector_type(2)));
-      const u2 l = __builtin_bit_cast(u2, lo), h2 = __builtin_bit_cast(u2, hi);
-      f[j] = u32x4_t{l[0], l[1], h2[0], h2[1]};
-    }
-  }
+// the fragment of 16-row block b of a staged tile, contraction half h
+template <typename T, int R, bool KC>
+__device__ __forceinline__ u32x4_t frag16(const char* lds, int b, int h, int n, int q) {
+  if (KC) return *reinterpret_cast<const u32x4_t*>(lds + (b * 16 + n) * 128 + (((h * 4 + q) ^ (n >> 1)) << 4));
+  const int sw = mn_swizzle<R>(8 * q + (n >> 2));  // (the same for all the contraction indices this lane addresses)
+  const char* a = lds + (h * 32 + 8 * q + (n >> 2)) * (R * 2) + (n & 3) * 8 + ((b ^ sw) << 5);
+  const s16x4 lo = read_transposed((lds_s16x4*)a), hi = read_transposed((lds_s16x4*)(a + 4 * R * 2));
+  typedef unsigned u2 __attribute__((ext_vector_type(2)));
+  const u2 l = __builtin_bit_cast(u2, lo), h2 = __builtin_bit_cast(u2, hi);
+  return u32x4_t{l[0], l[1], h2[0], h2[1]};
 }
 
 // s_waitcnt vmcnt(N) lgkmcnt(0), as the builtin (the compiler's own counting then knows of it), and the barrier, with nothing moved across
@@ -304,35 +293,58 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void gemm16_kernel(Gemm16<T> G) {
   for (int i = 0; i < RB; ++i)
 #pragma unroll
     for (int j = 0; j < CB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  auto load = [&](char* to) {
-    ta.load(to, wave);
-    tb.load(to + TA::BYTES, wave);
-  };
   auto load_any = [&](char* to, int s) {           // step s of this workgroup, which may be the contraction's last
     const int left = G.K - (s0 + s) * BK;
-    if (left >= BK) load(to);
-    else {
+    if (left >= BK) {
+#pragma unroll
+      for (int i = 0; i < TA::NI; ++i) ta.issue(to, wave, i);
+#pragma unroll
+      for (int i = 0; i < TB::NI; ++i) tb.issue(to + TA::BYTES, wave, i);
+      ta.advance();
+      tb.advance();
+    } else {
       ta.load_edge(to, KA ? (left + 7) & ~7 : left, lane, wave);
       tb.load_edge(to + TA::BYTES, KB ? (left + 7) & ~7 : left, lane, wave);
     }
   };
   u32x4_t fa0[RB], fb0[CB], fa1[RB], fb1[CB];
-  auto fetch = [&](const char* from, int h, u32x4_t (&a)[RB], u32x4_t (&b)[CB]) {
-    frags16<T, BM, RB, KA>(from, wr * RB, h, n, q, a);
-    frags16<T, BN, CB, KB>(from + TA::BYTES, wc * CB, h, n, q, b);
+  // reads half h of the tiles at `from`; with `to`, a whole step's DMA goes between the reads
+  auto fetch = [&](const char* from, int h, u32x4_t (&a)[RB], u32x4_t (&b)[CB], auto dma, char* to) {
+#pragma unroll
+    for (int i = 0; i < RB + CB; ++i) {
+      if (i < RB) a[i] = frag16<T, BM, KA>(from, wr * RB + i, h, n, q);
+      else b[i - RB] = frag16<T, BN, KB>(from + TA::BYTES, wc * CB + i - RB, h, n, q);
+      if constexpr (decltype(dma)::value) {
+#pragma unroll
+        for (int k = i * NI / (RB + CB); k < (i + 1) * NI / (RB + CB); ++k) {
+          if (k < TA::NI) ta.issue(to, wave, k);
+          else tb.issue(to + TA::BYTES, wave, k - TA::NI);
+        }
+      }
+    }
+    if constexpr (decltype(dma)::value) {
+      ta.advance();
+      tb.advance();
+    }
   };
-  auto multiply = [&](const u32x4_t (&a)[RB], const u32x4_t (&b)[CB]) {
+  auto multiply = [&](const u32x4_t (&a)[RB], const u32x4_t (&b)[CB], auto dma) {
 #pragma unroll
     for (int i = 0; i < RB; ++i)
 #pragma unroll
       for (int j = 0; j < CB; ++j) acc[i][j] = mfma16x32(b[j], a[i], acc[i][j], G.A);
-    constexpr int NR = (KA ? RB : 2 * RB) + (KB ? CB : 2 * CB), PER = RB * CB / NR > 0 ? RB * CB / NR : 1;
+    constexpr int NR = RB + CB, PER = RB * CB / NR > 0 ? RB * CB / NR : 1;
 #pragma unroll
-    for (int k = 0; k < NR; ++k) {                 // the reads spread between the products
+    for (int k = 0; k < NR; ++k) {                 // the reads and the DMA spread between the products
       __builtin_amdgcn_sched_group_barrier(0x008, PER, 0);
-      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      if (k < RB ? KA : KB) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      else __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      if constexpr (decltype(dma)::value) {
+        if ((k + 1) * NI / NR > k * NI / NR) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+      }
     }
   };
+  constexpr std::true_type with_dma{};
+  constexpr std::false_type no_dma{};
   char *cur = lds, *nxt = lds + SB;
   auto advance = [&] {
     cur = nxt;
@@ -343,26 +355,25 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void gemm16_kernel(Gemm16<T> G) {
     if (k < steps) load_any(lds + k * SB, k);
   if (steps >= ST) wait_and_meet<NI * (ST - 1)>();
   else wait_and_meet<0>();
-  fetch(cur, 0, fa0, fb0);
+  fetch(cur, 0, fa0, fb0, no_dma, nullptr);
   int s = 0;
   for (; s + ST + 1 < steps; ++s) {                // (steps that load whole ones)
-    fetch(cur, 1, fa1, fb1);
-    multiply(fa0, fb0);
+    fetch(cur, 1, fa1, fb1, no_dma, nullptr);
+    multiply(fa0, fb0, no_dma);
     wait_and_meet<NI * (ST - 2)>();
-    load(cur);
-    fetch(nxt, 0, fa0, fb0);
-    multiply(fa1, fb1);
+    fetch(nxt, 0, fa0, fb0, with_dma, cur);
+    multiply(fa1, fb1, with_dma);
     advance();
   }
 #pragma unroll 1
   for (; s < steps; ++s) {                         // the last ST + 1: the contraction's end may be in what they load
-    fetch(cur, 1, fa1, fb1);
-    multiply(fa0, fb0);
+    fetch(cur, 1, fa1, fb1, no_dma, nullptr);
+    multiply(fa0, fb0, no_dma);
     if (s + ST - 1 < steps) wait_and_meet<NI * (ST - 2)>();
     else wait_and_meet<0>();
     if (s + ST < steps) load_any(cur, s + ST);
-    fetch(nxt, 0, fa0, fb0);                       // (past the last step: values that nothing uses)
-    multiply(fa1, fb1);
+    fetch(nxt, 0, fa0, fb0, no_dma, nullptr);      // (past the last step: values that nothing uses)
+    multiply(fa1, fb1, no_dma);
     advance();
   }
   // The results leave through LDS, 16 rows of every wave at a time: a thread then has eight consecutive columns, the same ones in every
@@ -494,29 +505,38 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void gemm16_few_kernel(Gemm16<T> G)
     for (int e = 0; e < 8; ++e) f[e] = k + e < G.K ? to_f(p[e]) : 0.f;
     return vpack(f, p);
   };
-  for (int k0 = wave * 128; k0 < G.K; k0 += FEW_WAVES * 128) {
-    if (k0 + 128 <= G.K) {
-      u32x4_t w[4], x[MB][4];
+  u32x4_t w[2][4], x[2][MB][4];                    // a stretch's operands and, on their way, the next one's
+  auto load = [&](int k0, u32x4_t (&w)[4], u32x4_t (&x)[MB][4]) {
 #pragma unroll
-      for (int s = 0; s < 4; ++s) w[s] = ld16(wp + k0 + 32 * s);
+    for (int s = 0; s < 4; ++s) w[s] = ld16(wp + k0 + 32 * s);
 #pragma unroll
-      for (int m = 0; m < MB; ++m)
+    for (int m = 0; m < MB; ++m)
 #pragma unroll
-        for (int s = 0; s < 4; ++s) x[m][s] = ld16(xp[m] + k0 + 32 * s);
+      for (int s = 0; s < 4; ++s) x[m][s] = ld16(xp[m] + k0 + 32 * s);
+  };
+  auto multiply = [&](const u32x4_t (&w)[4], const u32x4_t (&x)[MB][4]) {
 #pragma unroll
-      for (int s = 0; s < 4; ++s)
+    for (int s = 0; s < 4; ++s)
 #pragma unroll
-        for (int m = 0; m < MB; ++m) acc[m] = mfma16x32(w[s], x[m][s], acc[m], G.A);
-    } else {
-      for (int k = k0; k < G.K; k += 32) {
-        const int kl = k + 8 * q;
-        const u32x4_t w = kl + 8 <= G.K ? ld16(wp + k) : tail8(wp + k, kl);
+      for (int m = 0; m < MB; ++m) acc[m] = mfma16x32(w[s], x[m][s], acc[m], G.A);
+  };
+  constexpr int STRIDE = FEW_WAVES * 128;
+  int k0 = wave * 128;
+  if (k0 + 128 <= G.K) load(k0, w[0], x[0]);
+  for (; k0 + 128 <= G.K; k0 += 2 * STRIDE) {
+    if (k0 + STRIDE + 128 <= G.K) load(k0 + STRIDE, w[1], x[1]);
+    multiply(w[0], x[0]);
+    if (k0 + STRIDE + 128 > G.K) { k0 += STRIDE; break; }
+    if (k0 + 2 * STRIDE + 128 <= G.K) load(k0 + 2 * STRIDE, w[0], x[0]);
+    multiply(w[1], x[1]);
+  }
+  for (int k = k0; k < G.K && k < k0 + 128; k += 32) {         // the contraction's end, if it lies in this wave's last stretch
+    const int kl = k + 8 * q;
+    const u32x4_t we = kl + 8 <= G.K ? ld16(wp + k) : tail8(wp + k, kl);
 #pragma unroll
-        for (int m = 0; m < MB; ++m) {
-          const u32x4_t x = kl + 8 <= G.K ? ld16(xp[m] + k) : tail8(xp[m] + k, kl);
-          acc[m] = mfma16x32(w, x, acc[m], G.A);
-        }
-      }
+    for (int m = 0; m < MB; ++m) {
+      const u32x4_t xe = kl + 8 <= G.K ? ld16(xp[m] + k) : tail8(xp[m] + k, kl);
+      acc[m] = mfma16x32(we, xe, acc[m], G.A);
     }
   }
 #pragma unroll
@@ -651,11 +671,10 @@ static constexpr Form16 FORMS16[] = {{256, 256, 256, 8.f, 1.55f, 1.55f, 1.f},   
                                      {128, 128, 512, 4.5f, 0.62f, 0.89f, 2.5f},
                                      {128, 128, 256, 5.f, 0.47f, 0.47f, 1.5f},    // four buffers: one workgroup per CU, DMA three steps ahead
                                      {64, 64, 512, 3.f, 0.18f, 0.35f, 0.8f}};
-struct Plan16 { int form, tiles_m, tiles_n, splits; };
+struct Plan16 { int form, tiles_m, tiles_n, splits; float us; };
 static Plan16 plan16(int M, int N, int K, int layout) {
   const int steps = (K + G16_BK - 1) / G16_BK;
-  Plan16 best{0, 0, 0, 0};
-  float least = 0.f;
+  Plan16 best{0, 0, 0, 0, 0.f};
   for (int f = 0; f < 5; ++f) {
     if (f == 1 && layout == 2) continue;
     const Form16& F = FORMS16[f];
@@ -667,13 +686,17 @@ static Plan16 plan16(int M, int N, int K, int layout) {
       float t = F.start + (float)rounds * (n * F.together + F.end);
       if (rest > 0) t += n * (rest > 256 ? F.together : F.alone) + F.end;
       if (sp > 1) t += 4.f + 8.f * (float)sp * (float)M * (float)N / 12e6f;
-      if (best.splits == 0 || t < least) {
-        least = t;
-        best = Plan16{f, (int)tm, (int)tn, sp};
-      }
+      if (best.splits == 0 || t < best.us) best = Plan16{f, (int)tm, (int)tn, sp, t};
     }
   }
   return best;
+}
+
+// Up to 64 rows of x w^T: the few-row form where the model finds it faster (one row of 4096 x 4096: 7.0 us against 8.9 in tiles; 64 rows: 20.4
+// against 12.3; 64 rows of 768 x 768 5.2 against 5.8), and wherever the operands do not lie as tiles need them.
+static bool few16(int M, int N, int K, const Plan16& p) {
+  const float per_k = M <= 16 ? 1.6e-3f : M <= 32 ? 2.4e-3f : 4.2e-3f;
+  return 3.f + (float)((N + 16 * 512 - 1) / (16 * 512)) * (float)K * per_k <= p.us;
 }
 
 template <typename T, int BM, int BN, int WR, int WC, int ST, bool KA, bool KB> static void gemm16_go(const Gemm16<T>& G, hipStream_t st) {
@@ -683,15 +706,14 @@ template <typename T, int BM, int BN, int WR, int WC, int ST, bool KA, bool KB> 
   (void)once;
   hipLaunchKernelGGL(k, dim3((unsigned)(G.tiles_m * G.tiles_n * G.splits)), dim3(64 * WR * WC), bytes, st, G);
 }
-template <typename T> static void gemm16_run(Gemm16<T> G, int layout, float* ws, hipStream_t st) {
-  if (layout == 0 && G.M <= FEW_ROWS) {
+template <typename T> static void gemm16_run(Gemm16<T> G, int layout, bool few, const Plan16& p, float* ws, hipStream_t st) {
+  if (few) {
     const dim3 grid((G.N + 15) / 16), block(64 * FEW_WAVES);
     if (G.M <= 16) hipLaunchKernelGGL((gemm16_few_kernel<T, 1>), grid, block, 0, st, G);
     else if (G.M <= 32) hipLaunchKernelGGL((gemm16_few_kernel<T, 2>), grid, block, 0, st, G);
     else hipLaunchKernelGGL((gemm16_few_kernel<T, 4>), grid, block, 0, st, G);
     return;
   }
-  const Plan16 p = plan16(G.M, G.N, G.K, layout);
   G.tiles_m = p.tiles_m;
   G.tiles_n = p.tiles_n;
   G.splits = p.splits;
@@ -731,8 +753,8 @@ using namespace hopmi;
 
 extern "C" size_t hopmi_gemm16_ws_floats(int M, int N, int K, int layout) {
   if (M < 1 || N < 1 || K < 1 || layout < 0 || layout > 2) return 0;
-  if (layout == 0 && M <= FEW_ROWS) return 0;
   const Plan16 p = plan16(M, N, K, layout);
+  if (layout == 0 && M <= FEW_ROWS && few16(M, N, K, p)) return 0;
   return p.splits > 1 ? (size_t)p.splits * M * N : 0;
 }
 
@@ -750,12 +772,15 @@ extern "C" int hopmi_gemm16(const void* A, long long lda, const void* B, long lo
   const int ca = layout == 2 ? M : K, cb = layout == 0 ? K : N;
   if (lda < ca || ldb < cb || ldc < N || (res && ldr < N) || (z && ldz < N)) { set_error("hopmi_gemm16: a row stride below the row's length"); return HOPMI_EINVAL; }
   if (lda > (1 << 22) || ldb > (1 << 22)) { set_error("hopmi_gemm16: row stride above 2^22 elements"); return HOPMI_EINVAL; }
-  const bool few = layout == 0 && M <= FEW_ROWS;
-  if (!few && (!g16_direct(A, lda, 0) || !g16_direct(B, ldb, 0) || lda < ((ca + 7) & ~7) || ldb < ((cb + 7) & ~7))) {
+  const Plan16 p = plan16(M, N, K, layout);
+  const bool tiled = g16_direct(A, lda, 0) && g16_direct(B, ldb, 0) && lda >= ((ca + 7) & ~7) && ldb >= ((cb + 7) & ~7);
+  // (rows whose last vector is not whole may be followed by anything where rows run along the contraction: the few-row form then)
+  const bool few = layout == 0 && M <= FEW_ROWS && (!tiled || (K & 7) || few16(M, N, K, p));
+  if (!few && !tiled) {
     set_error("hopmi_gemm16: operands need rows on 16 bytes that end on 16 bytes (hopmi_pad16)");
     return HOPMI_EINVAL;
   }
-  if (!few && hopmi_gemm16_ws_floats(M, N, K, layout) > 0 && !ws) { set_error("hopmi_gemm16: null workspace"); return HOPMI_EINVAL; }
+  if (!few && p.splits > 1 && !ws) { set_error("hopmi_gemm16: null workspace"); return HOPMI_EINVAL; }
   hipStream_t st = static_cast<hipStream_t>(stream);
   auto go = [&](auto t) {
     using T = decltype(t);
@@ -765,7 +790,7 @@ extern "C" int hopmi_gemm16(const void* A, long long lda, const void* B, long lo
     G.M = M; G.N = N; G.K = K;
     G.E = Epi16<T>{static_cast<T*>(C), ldc, static_cast<const T*>(bias), static_cast<const T*>(res), ldr, static_cast<T*>(z), ldz, act};
     G.part = nullptr; G.tiles_m = G.tiles_n = G.splits = 1;
-    gemm16_run(G, layout, ws, st);
+    gemm16_run(G, layout, few, p, ws, st);
   };
   if (dtype == T_BF16) go(__bf16{}); else go(_Float16{});
   return check_launch("hopmi_gemm16");

@@ -66,7 +66,7 @@ def test_gemm16_entry_points_refuse():
         assert call(**kw) == -1 and "16 bytes" in _last(), kw
     assert L.hopmi_gemm16_ws_floats(128, 128, 4096, 0) > 0
     assert call(K=4096, lda=4096, ldb=4096, ws=None) == -1 and "workspace" in _last()
-    assert L.hopmi_gemm16_ws_floats(64, 128, 4096, 0) == 0 and L.hopmi_gemm16_ws_floats(0, 1, 1, 0) == 0
+    assert L.hopmi_gemm16_ws_floats(16, 128, 768, 0) == 0 and L.hopmi_gemm16_ws_floats(0, 1, 1, 0) == 0
     assert L.hopmi_gemm16_direct(ONE, 64, 64) == 1 and L.hopmi_gemm16_direct(ONE, 64, 60) == 0 and L.hopmi_gemm16_direct(ctypes.c_void_p(8), 64, 64) == 0
     assert L.hopmi_pad16(ONE, 5, ONE, 12, 4, 5, None) == -1 and L.hopmi_pad16(ONE, 5, ctypes.c_void_p(8), 8, 4, 5, None) == -1
     for kw in (dict(act=2, z=None), dict(ldz=12), dict(ws=None), dict(ldd=12), dict(dt=0)):

@@ -248,9 +248,9 @@ def _check_linear(M, K, N, t, act, bias, res, backward, seed=0, mk=None):
 
 # few rows (each number of 16-row blocks, odd contraction ends), the first row counts of the tiled form, odd sides, one and several
 # k-steps, contraction tails (64 n + 8 m and odd), split contractions, one column
-LIN_SIZES = [(1, 1, 1), (1, 768, 2304), (2, 3, 5), (16, 33, 17), (17, 64, 16), (33, 129, 40), (34, 768, 768), (64, 130, 50), (64, 4096, 19),
+LIN_SIZES = [(64, 4096, 72), (48, 4096, 4096), (33, 2048, 136), (1, 1, 1), (1, 768, 2304), (2, 3, 5), (16, 33, 17), (17, 64, 16), (33, 129, 40), (34, 768, 768), (64, 130, 50), (64, 4096, 19),
              (65, 64, 64), (65, 72, 40), (66, 7, 9), (129, 100, 33), (100, 1, 130), (300, 1021, 427), (512, 768, 256), (130, 4160, 136),
-             (1000, 200, 1)]
+             (1000, 200, 1), (260, 4352, 200), (1024, 1024, 1030), (2176, 768, 770)]
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
