@@ -20,3 +20,4 @@ from .graph import GraphedTrainStep                   # noqa: F401
 from .feeder import HostFeeder, log_melspec           # noqa: F401
 from .tuning import use_tuned_gemms                   # noqa: F401
 from .ops import gemm_parts, strict_fp32              # noqa: F401
+from .ops import layer_norm, LayerNorm, linear_act, GradClip, clip_grad_norm_   # noqa: F401

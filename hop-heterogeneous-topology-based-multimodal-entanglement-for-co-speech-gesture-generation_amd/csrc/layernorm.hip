@@ -3,7 +3,9 @@
 //   mu = sum_d x / D      v = sum_d (x - mu)^2 / D      r = 1 / sqrt(v + eps)      xh = (x - mu) r      y = xh g + b
 //   dx = r (g dy - mean_d(g dy) - xh mean_d(g dy xh))       dg = sum_rows dy xh       db = sum_rows dy
 //
-// Bound: HBM (8 / 22 operations per element against 4-8 / 6-12 bytes).  So each pass reads x (and dy) once: a row stays in the
+// Bound: HBM (8 / 22 operations per element against 4-8 / 6-12 bytes); measured, in a recorded graph: forward 8192 x 4096 fp32 41.8 us (6.5 TB/s
+// of x and y together, some of it from the 256 MB cache), backward 85.6 (4.7 TB/s of x, dy, dx); 32768 x 1024 bf16 22.4 and 41.0; a large copy
+// moves 5.2 TB/s.  Below some 10 MB the launches bound it: 4352 x 768 bf16 5.0 and 12.9 us (two launches), one window of 34 rows 3.0.  So each pass reads x (and dy) once: a row stays in the
 // registers of one wave (up to 256 16-byte vectors) or of a workgroup of 256 (up to 512), 512 (1024) or 1024 threads (2048);
 // wider rows are re-read (from the caches) by the looped form.  The variance is taken around the mean, not as E x^2 - mu^2: the row
 // is in registers, a second pass over it costs no memory.
@@ -160,7 +162,7 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void ln_bwd_kernel(const T* 
                                                                        float* __restrict__ part, int M, int D) {
   constexpr int V = Vec<T>::N, RPB = TPR == 64 ? 4 : 1;
   __shared__ float xch[4 * (TPR / 64)];
-  extern __shared__ float comb[];                            // TPR == 64: [3][2][D], the other waves' column sums
+  extern __shared__ float comb[];                            // TPR == 64: [4][2][D], the waves' column sums
   int phase = 0;
   const int lane = threadIdx.x & (TPR - 1), vecs = D / V, tail = D - vecs * V, td = vecs * V + lane;
   const float invD = 1.f / (float)D;
@@ -258,16 +260,11 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void ln_bwd_kernel(const T* 
         for (int e = 0; e < V; ++e) f((lane + TPR * i) * V + e, dg[i][e], db[i][e]);
     if (lane < tail) f(td, dgt, dbt);
   };
-  if (TPR == 64) {
-    const int wave = threadIdx.x >> 6;
-    if (wave > 0) visit([&](int d, float a, float c) { comb[(wave - 1) * 2 * D + d] = a; comb[(wave - 1) * 2 * D + D + d] = c; });
+  if (TPR == 64) {                                           // the four waves' sums meet in LDS, all threads add
+    float* mine = comb + (threadIdx.x >> 6) * 2 * D;
+    visit([&](int d, float a, float c) { mine[d] = a; mine[D + d] = c; });
     __syncthreads();
-    if (wave > 0) return;
-    visit([&](int d, float a, float c) {
-      for (int k = 0; k < 3; ++k) { a += comb[k * 2 * D + d]; c += comb[k * 2 * D + D + d]; }
-      out[d] = a;
-      out[D + d] = c;
-    });
+    for (int d = threadIdx.x; d < 2 * D; d += 256) out[d] = comb[d] + comb[2 * D + d] + comb[4 * D + d] + comb[6 * D + d];
   } else {
     visit([&](int d, float a, float c) { out[d] = a; out[D + d] = c; });
   }
@@ -355,11 +352,14 @@ static int ln_form(int D, int dtype) {
   const int vecs = D / (dtype == T_F32 ? 4 : 8);
   return vecs <= 256 ? 64 : vecs <= 512 ? 256 : vecs <= 1024 ? 512 : vecs <= 2048 ? 1024 : 0;
 }
-// workgroups of a backward launch: rows in whole passes over an even grid of at most 512 workgroups
-static int ln_bwd_grid(int M, int form) {
+// Workgroups of a backward launch: rows in whole passes over an even grid.  More workgroups hide more latency and leave more partial rows:
+// up to 1024 where a row is 128 vectors or fewer (32768 x 1024 bf16: 41.0 us against 44.0 on 512; 65536 x 256 fp32 36.6 / 45.0; 4352 x 768 bf16
+// 12.9 / 13.8), up to 512 for wider ones (16384 x 2048 bf16: 45.2 us against 54.7 on 1024; 8192 x 4096 fp32 85.6 / 90.2).
+static int ln_bwd_grid(int M, int D, int dtype) {
+  const int form = ln_form(D, dtype), cap = D / (dtype == T_F32 ? 4 : 8) <= 128 ? 1024 : 512;
   const long long units = form == 64 ? ((long long)M + 3) / 4 : M;
   if (form == 0) return (int)(units < 64 ? units : 64);
-  const long long passes = (units + 511) / 512;
+  const long long passes = (units + cap - 1) / cap;
   return (int)((units + passes - 1) / passes);
 }
 
@@ -389,9 +389,12 @@ static void ln_fwd_typed(const void* x, long long ldx, const void* w, const void
 
 template <typename T, typename WT, int NV, int TPR>
 static void ln_bwd_go(const void* x, long long ldx, const void* dy, const float* mean, const float* rstd, const void* w, void* dx,
-                      float* part, int M, int D, hipStream_t st) {
-  hipLaunchKernelGGL((ln_bwd_kernel<T, WT, NV, TPR>), dim3(ln_bwd_grid(M, TPR)), dim3(TPR == 64 ? 256 : TPR),
-                     TPR == 64 && part != nullptr ? 3 * 2 * D * sizeof(float) : 0, st, static_cast<const T*>(x), ldx,
+                      float* part, int M, int D, int grid, hipStream_t st) {
+  const auto k = ln_bwd_kernel<T, WT, NV, TPR>;
+  const size_t lds = TPR == 64 && part != nullptr ? 8 * D * sizeof(float) : 0;               // up to 66 KB
+  static const hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, 72 * 1024);
+  (void)once;
+  hipLaunchKernelGGL(k, dim3(grid), dim3(TPR == 64 ? 256 : TPR), lds, st, static_cast<const T*>(x), ldx,
                      static_cast<const T*>(dy), mean, rstd, static_cast<const WT*>(w), static_cast<T*>(dx), part, M, D);
 }
 
@@ -399,18 +402,18 @@ template <typename T, typename WT>
 static void ln_bwd_typed(const void* x, long long ldx, const void* dy, const float* mean, const float* rstd, const void* w,
                          void* dx, float* part, int M, int D, int dtype, hipStream_t st) {
   const int vecs = D / Vec<T>::N, form = ln_form(D, dtype);
-  if (form == 64 && vecs <= 64) ln_bwd_go<T, WT, 1, 64>(x, ldx, dy, mean, rstd, w, dx, part, M, D, st);
-  else if (form == 64 && vecs <= 128) ln_bwd_go<T, WT, 2, 64>(x, ldx, dy, mean, rstd, w, dx, part, M, D, st);
-  else if (form == 64) ln_bwd_go<T, WT, 4, 64>(x, ldx, dy, mean, rstd, w, dx, part, M, D, st);
-  else if (form == 256) ln_bwd_go<T, WT, 2, 256>(x, ldx, dy, mean, rstd, w, dx, part, M, D, st);
-  else if (form == 512) ln_bwd_go<T, WT, 2, 512>(x, ldx, dy, mean, rstd, w, dx, part, M, D, st);
-  else if (form == 1024) ln_bwd_go<T, WT, 2, 1024>(x, ldx, dy, mean, rstd, w, dx, part, M, D, st);
+  if (form == 64 && vecs <= 64) ln_bwd_go<T, WT, 1, 64>(x, ldx, dy, mean, rstd, w, dx, part, M, D, ln_bwd_grid(M, D, dtype), st);
+  else if (form == 64 && vecs <= 128) ln_bwd_go<T, WT, 2, 64>(x, ldx, dy, mean, rstd, w, dx, part, M, D, ln_bwd_grid(M, D, dtype), st);
+  else if (form == 64) ln_bwd_go<T, WT, 4, 64>(x, ldx, dy, mean, rstd, w, dx, part, M, D, ln_bwd_grid(M, D, dtype), st);
+  else if (form == 256) ln_bwd_go<T, WT, 2, 256>(x, ldx, dy, mean, rstd, w, dx, part, M, D, ln_bwd_grid(M, D, dtype), st);
+  else if (form == 512) ln_bwd_go<T, WT, 2, 512>(x, ldx, dy, mean, rstd, w, dx, part, M, D, ln_bwd_grid(M, D, dtype), st);
+  else if (form == 1024) ln_bwd_go<T, WT, 2, 1024>(x, ldx, dy, mean, rstd, w, dx, part, M, D, ln_bwd_grid(M, D, dtype), st);
   else {
     if (dx != nullptr)
       hipLaunchKernelGGL((ln_bwd_loop_kernel<T, WT>), dim3(M < 512 ? M : 512), dim3(1024), 0, st, static_cast<const T*>(x), ldx,
                          static_cast<const T*>(dy), mean, rstd, static_cast<const WT*>(w), static_cast<T*>(dx), M, D);
     if (part != nullptr)
-      hipLaunchKernelGGL((ln_bwd_cols_kernel<T>), dim3((D + 63) / 64, ln_bwd_grid(M, 0)), dim3(256), 0, st, static_cast<const T*>(x), ldx,
+      hipLaunchKernelGGL((ln_bwd_cols_kernel<T>), dim3((D + 63) / 64, ln_bwd_grid(M, D, dtype)), dim3(256), 0, st, static_cast<const T*>(x), ldx,
                          static_cast<const T*>(dy), mean, rstd, part, M, D);
   }
 }
@@ -451,7 +454,7 @@ extern "C" int hopmi_layernorm_fwd(const void* x, long long ldx, const void* wei
 
 extern "C" size_t hopmi_layernorm_bwd_ws_floats(int M, int D, int dtype) {
   if (M < 1 || D < 1 || dtype < T_F32 || dtype > T_F16) return 0;
-  return (size_t)ln_bwd_grid(M, ln_form(D, dtype)) * 2 * D;
+  return (size_t)ln_bwd_grid(M, D, dtype) * 2 * D;
 }
 
 extern "C" int hopmi_layernorm_bwd(const void* x, long long ldx, const void* dy, const float* mean, const float* rstd, const void* weight,
@@ -467,7 +470,7 @@ extern "C" int hopmi_layernorm_bwd(const void* x, long long ldx, const void* dy,
     using WT = decltype(wt);
     ln_bwd_typed<decltype(t), WT>(x, ldx, dy, mean, rstd, weight, dx, part, M, D, dtype, st);
     if (sums)
-      hipLaunchKernelGGL((ln_reduce_kernel<WT>), dim3((2 * D + 63) / 64), dim3(1024), 0, st, part, ln_bwd_grid(M, ln_form(D, dtype)), D,
+      hipLaunchKernelGGL((ln_reduce_kernel<WT>), dim3((2 * D + 63) / 64), dim3(1024), 0, st, part, ln_bwd_grid(M, D, dtype), D,
                          static_cast<WT*>(dweight), static_cast<WT*>(dbias));
   });
   return check_launch("hopmi_layernorm_bwd");

@@ -31,6 +31,7 @@ import gc
 import torch
 import torch.distributed as dist
 
+from . import _lib
 from . import ops as _ops
 from . import steps as _steps
 
@@ -262,6 +263,9 @@ class GraphedTrainStep:
         self.world = dist.get_world_size(group) if dist.is_available() and dist.is_initialized() else 1
         self.rank = dist.get_rank(group) if self.world > 1 else 0
         self.exchange = self.world > 1 or (force_exchange and dist.is_available() and dist.is_initialized())
+        if self.exchange and getattr(args, "max_grad_norm", None) is not None:
+            raise _lib.HopmiError("hopmi GraphedTrainStep: max_grad_norm needs every rank to hold the whole gradient, and the recorded step shards "
+                                  "the mapping layer's rows over the ranks; steps.train_llm with a GradSync clips")
         self.accel = accelerator if accelerator is not None else _PlainBackward()
         # at least one eager call per phase: besides library handles, every model builds state lazily in its first call
         # (the frozen BERT's operand images, the GRU's packed weights, selection matrices), and some of that cannot be recorded
@@ -550,7 +554,6 @@ class GraphedTrainStep:
         import os
         import sys
         import traceback
-        from . import _lib
         print("hopmi GraphedTrainStep: exception while recording the step:", file=sys.stderr)
         traceback.print_exception(type(exc), exc, exc.__traceback__, file=sys.stderr)
         self.enabled = False
@@ -606,7 +609,8 @@ class GraphedTrainStep:
         if left > 0:
             self.eager_left[gan] = left - 1
             return self._eager(epoch, batch)
-        key = (gan, torch.is_autocast_enabled(), _steps._MIXED, getattr(self.args, "mixed_precision", None)) + tuple(
+        key = (gan, torch.is_autocast_enabled(), _steps._MIXED, getattr(self.args, "mixed_precision", None),
+               getattr(self.args, "max_grad_norm", None)) + tuple(
             (tuple(t.shape), t.dtype) for t in batch)
         rec = self.records.get(key)
         if rec is not None and rec["frozen"] != self._frozen_versions():

@@ -93,6 +93,14 @@ def _regularisers(args, outputs, z_context, z_mu, z_logvar, out_rand, z_rand):
     return div_reg, kld
 
 
+def _clip(args, optim):
+    """`args.max_grad_norm` (absent or None: no clipping, as the reference trains): the generator's gradients scaled to that global
+    2-norm in front of its optimizer step (ops.clip_grad_norm_; nothing is read back)."""
+    limit = getattr(args, "max_grad_norm", None)
+    if limit is not None:
+        _ops.clip_grad_norm_([p for g in optim.param_groups for p in g["params"]], limit)
+
+
 _CAPTURE = None     # a graph._Capture while a training-step graph is being recorded (see graph.GraphedTrainStep)
 
 
@@ -283,6 +291,7 @@ def train_llm(args, epoch, in_audio, log_melspec, text_token_padded, target_dir_
                 loss = loss + gen_error * args.loss_gan_weight
         fetch = _LossFetch(args, gan, huber_loss, kld, div_reg, gen_error, dis_error)
         _backward(accelerator, loss, model)
+        _clip(args, model_optim)
         model_optim.step()
     return fetch.result()
 
@@ -328,5 +337,6 @@ def train_iter_gan(args, epoch, in_text, in_audio, target_poses, vid_indices,
         loss = loss + args.loss_gan_weight * gen_error
     fetch = _LossFetch(args, gan, huber_loss, kld, div_reg, gen_error, dis_error)
     loss.backward()
+    _clip(args, pose_dec_optim)
     pose_dec_optim.step()
     return fetch.result()

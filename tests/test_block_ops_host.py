@@ -89,3 +89,22 @@ def test_grad_clip_entry_point_refuses():
     many = 250 * 129
     assert L.hopmi_grad_clip((ctypes.c_void_p * many)(*[16] * many), None, (ctypes.c_longlong * many)(*[1] * many),
                              (ctypes.c_int * many)(), many, 1.0, ONE, ONE, None) == -1 and "more than one call" in _last()
+
+
+def test_recorded_step_over_ranks_refuses_max_grad_norm(tmp_path):
+    """The recorded step shards the mapping layer's gradient over the ranks: no rank has the norm."""
+    import types
+
+    import torch.distributed as dist
+    mod = torch.nn.Linear(2, 2)
+    args = types.SimpleNamespace(max_grad_norm=1.0)
+    assert not hopmi.GraphedTrainStep(args, mod, mod, None, None).exchange            # one rank: accepted
+    if dist.is_initialized():
+        pytest.skip("a process group is up in this process")
+    dist.init_process_group("gloo", init_method=f"file://{tmp_path}/store", rank=0, world_size=1)
+    try:
+        with pytest.raises(_lib.HopmiError, match="max_grad_norm"):
+            hopmi.GraphedTrainStep(args, mod, mod, None, None, force_exchange=True)
+        assert hopmi.GraphedTrainStep(types.SimpleNamespace(), mod, mod, None, None, force_exchange=True).exchange
+    finally:
+        dist.destroy_process_group()

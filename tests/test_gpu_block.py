@@ -593,3 +593,41 @@ def test_block_step_captured_and_replayed():
         torch.cuda.synchronize()
         for w, (*_, r) in zip(want, (a, b)):
             assert all(torch.equal(p, q) for p, q in zip(w, r)), k
+
+
+@pytest.mark.parametrize("recorded", [False, True])
+def test_training_step_clips_by_max_grad_norm(recorded, monkeypatch):
+    """args.max_grad_norm: train_llm, eager and recorded, steps on gradients of that global norm (the gradients that a step leaves behind
+    are the ones its optimizer read), and a limit above the norm changes no bit."""
+    import copy
+    from oracle.golden_util import Accel, step_args
+    from test_gpu_graph import _deterministic_draws, _pair
+    _deterministic_draws(monkeypatch)
+    m0, d0, inp = _pair(9, _dev())
+    batch = (inp["in_audio"], inp["log_melspec"], inp["text"], inp["target_dir_vec"], inp["vid_indices"])
+
+    def steps(limit, n):
+        m, d = copy.deepcopy(m0), copy.deepcopy(d0)
+        m._randn_like = m0._randn_like
+        g = torch.optim.Adam([p for p in m.parameters() if p.requires_grad], lr=1e-4, betas=(0.5, 0.999))
+        o = torch.optim.Adam(d.parameters(), lr=1e-4, betas=(0.5, 0.999))
+        args = step_args(9)
+        if limit is not None:
+            args.max_grad_norm = limit
+        run = hopmi.GraphedTrainStep(args, m, d, g, o, eager_calls=1) if recorded else lambda e, *b: hopmi.train_llm(args, e, *b, m, d, g, o, Accel())
+        for _ in range(n):
+            run(0, *batch)
+        torch.cuda.synchronize()
+        grads = [p.grad for p in m.parameters() if p.grad is not None]
+        assert grads and (not recorded or run.n_replay == n - 1)
+        return m, math.sqrt(sum(float(v.double().square().sum()) for v in grads))
+
+    free, norm = steps(None, 3)
+    same, _ = steps(1e6 * norm, 3)
+    assert all(torch.equal(p, q) for p, q in zip(free.parameters(), same.parameters()))
+    clipped, after = steps(0.125 * norm, 3)
+    # every step's norm stays far above the limit here, so the last step's gradients have it as their norm: 1e-6 in the formula's
+    # denominator and one rounding per value
+    assert abs(after - 0.125 * norm) <= 1e-5 * norm
+    assert not all(torch.equal(p, q) for p, q in zip(free.parameters(), clipped.parameters()))
+
