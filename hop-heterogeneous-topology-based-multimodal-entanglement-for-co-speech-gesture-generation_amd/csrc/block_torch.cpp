@@ -35,7 +35,7 @@ PyObject* g_error = nullptr;                       // _lib.HopmiError
 
 #define HOPMI_API(X)                                                                                                       \
   X(hopmi_last_error) X(hopmi_layernorm_fwd) X(hopmi_layernorm_bwd_ws_floats) X(hopmi_layernorm_bwd) X(hopmi_gemm16_ws_floats) \
-  X(hopmi_gemm16) X(hopmi_pad16) X(hopmi_act_bwd16_ws_floats) X(hopmi_act_bwd16) X(hopmi_grad_clip_ws_bytes) X(hopmi_grad_clip)
+  X(hopmi_gemm16) X(hopmi_gemm16_direct) X(hopmi_pad16) X(hopmi_act_bwd16_ws_floats) X(hopmi_act_bwd16) X(hopmi_grad_clip_ws_bytes) X(hopmi_grad_clip)
 struct Api {
 #define X(f) decltype(&::f) f = nullptr;
   HOPMI_API(X)
@@ -185,14 +185,13 @@ Tensor layer_norm(const Tensor& x, const OptTensor& w0, const OptTensor& b0, dou
 
 // ------------------------------------------------------------------------------------------------------------- linear_act
 constexpr int FEW_ROWS = 64;                       // up to here layout 0 takes operands of any alignment
-constexpr int64_t MAX_LD = int64_t(1) << 22;
+constexpr int64_t MOST = int64_t(1) << 22;         // longest row that the tiled products address
 
-bool direct(const Rows& r) { return !((reinterpret_cast<uintptr_t>(r.t.const_data_ptr()) & 15) | (r.ld & 7) | (r.n & 7)) && r.ld <= MAX_LD; }
+bool direct(const Rows& r) { return L.hopmi_gemm16_direct(r.t.const_data_ptr(), r.ld, r.n) != 0; }
 // as hopmi_gemm16 takes it: as it lies where its rows start and end on 16 bytes, else copied into rows padded with zeros
 Rows operand(const Rows& r) {
   if (direct(r)) return r;
   const int64_t ld = (int64_t(r.n) + 7) / 8 * 8;
-  if (ld > MAX_LD) refuse("linear_act: rows of ", r.n, " elements are more than the kernel addresses (2^22)");
   Rows p{at::empty({r.m, ld}, r.t.options()), ld, r.m, r.n};
   check(L.hopmi_pad16(r.t.const_data_ptr(), r.ld, out(p.t), ld, r.m, r.n, stream(r.t)), "hopmi_pad16");
   return p;
@@ -309,6 +308,7 @@ Tensor linear_act(const Tensor& x0, const Tensor& w0, const OptTensor& b0, const
     if (has(t) && t->scalar_type() != x.scalar_type()) refuse("linear_act: `", name, "` is ", t->scalar_type(), ", x ", x.scalar_type(), ": one type for all operands");
   if (x.dim() < 1 || w.dim() != 2 || w.size(1) != x.size(-1) || w.size(0) < 1 || w.size(1) < 1)
     refuse("linear_act: x ", x.sizes(), " and w ", w.sizes(), " (N, K) do not fit, or have an empty side");
+  if (w.size(0) > MOST || w.size(1) > MOST) refuse("linear_act: w ", w.sizes(), ": sides of up to 2^22");
   if (has(b) && (b->dim() != 1 || b->size(0) != w.size(0))) refuse("linear_act: bias has shape ", b->sizes(), ", w ", w.sizes());
   if (has(r)) {
     at::DimVector shape(x.sizes().begin(), x.sizes().end());
@@ -332,8 +332,8 @@ bool fills(const Tensor& t) { return t.is_contiguous() || t.is_non_overlapping_a
 
 struct ClipPlan {
   std::vector<Tensor> in, to;
-  std::vector<const void*> src;
-  std::vector<void*> dst;
+  mutable std::vector<const void*> src;              // (addresses are read again by every call)
+  mutable std::vector<void*> dst;
   std::vector<long long> n;
   std::vector<int> dt;
   bool into = false;
@@ -372,6 +372,12 @@ struct ClipPlan {
 
   Tensor clip(double max_norm) const {
     if (!(max_norm >= 0.0)) refuse("GradClip: max_norm=", max_norm);
+    for (size_t i = 0; i < in.size(); ++i) {
+      if (in[i].numel() != n[i] || code(in[i].scalar_type()) != dt[i] || (into && to[i].numel() != n[i]))
+        refuse("GradClip: tensors[", i, "] is not the tensor that the plan was made for any more");
+      src[i] = in[i].const_data_ptr();
+      if (into) dst[i] = to[i].mutable_data_ptr();
+    }
     const c10::DeviceGuard guard(in[0].device());
     at::NoGradGuard no_grad;
     const auto opt = at::TensorOptions().device(in[0].device());

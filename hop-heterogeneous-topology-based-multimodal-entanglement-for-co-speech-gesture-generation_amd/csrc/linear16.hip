@@ -678,9 +678,11 @@ static Plan16 plan16(int M, int N, int K, int layout) {
   for (int f = 0; f < 5; ++f) {
     if (f == 1 && layout == 2) continue;
     const Form16& F = FORMS16[f];
+    const int threads = f == 0 ? 512 : 256;
     const long long tm = ((long long)M + F.bm - 1) / F.bm, tn = ((long long)N + F.bn - 1) / F.bn, tiles = tm * tn;
     // (more splits than fill the chip once, or steps of fewer than four, never pay: the join reads every partial result again)
     for (int sp = 1; sp <= 32 && (sp == 1 || (tiles * sp <= F.slots && steps / sp >= 4)); sp += sp < 4 ? 1 : sp / 2) {
+      if (tiles * sp * threads >= 1LL << 32) break;          // (more than a launch counts)
       const long long wgs = tiles * sp, rounds = wgs / F.slots, rest = wgs - rounds * F.slots;
       const float n = (float)((steps + sp - 1) / sp);
       float t = F.start + (float)rounds * (n * F.together + F.end);
@@ -696,7 +698,7 @@ static Plan16 plan16(int M, int N, int K, int layout) {
 // against 12.3; 64 rows of 768 x 768 5.2 against 5.8), and wherever the operands do not lie as tiles need them.
 static bool few16(int M, int N, int K, const Plan16& p) {
   const float per_k = M <= 16 ? 1.6e-3f : M <= 32 ? 2.4e-3f : 4.2e-3f;
-  return 3.f + (float)((N + 16 * 512 - 1) / (16 * 512)) * (float)K * per_k <= p.us;
+  return p.splits == 0 || 3.f + (float)((N + 16 * 512 - 1) / (16 * 512)) * (float)K * per_k <= p.us;
 }
 
 template <typename T, int BM, int BN, int WR, int WC, int ST, bool KA, bool KB> static void gemm16_go(const Gemm16<T>& G, hipStream_t st) {
@@ -736,8 +738,9 @@ template <typename T> static void gemm16_run(Gemm16<T> G, int layout, bool few, 
   }
 }
 
+// rows of `cols` elements as tiles are staged from them: 16-byte addresses and ends, and a stride whose 256 rows an offset of 32 bits spans
 static bool g16_direct(const void* p, long long ld, int cols) {
-  return !((reinterpret_cast<uintptr_t>(p) & 15) | (ld & 7) | (cols & 7));
+  return !((reinterpret_cast<uintptr_t>(p) & 15) | (ld & 7) | (cols & 7)) && ld <= 1 << 22;
 }
 static int act_bwd_groups(int M, int N) {
   const int strips = (N + 511) / 512;
@@ -771,15 +774,15 @@ extern "C" int hopmi_gemm16(const void* A, long long lda, const void* B, long lo
   if (dtype != T_BF16 && dtype != T_F16) { set_error("hopmi_gemm16: dtype=%d (1 bf16, 2 fp16)", dtype); return HOPMI_EINVAL; }
   const int ca = layout == 2 ? M : K, cb = layout == 0 ? K : N;
   if (lda < ca || ldb < cb || ldc < N || (res && ldr < N) || (z && ldz < N)) { set_error("hopmi_gemm16: a row stride below the row's length"); return HOPMI_EINVAL; }
-  if (lda > (1 << 22) || ldb > (1 << 22)) { set_error("hopmi_gemm16: row stride above 2^22 elements"); return HOPMI_EINVAL; }
   const Plan16 p = plan16(M, N, K, layout);
   const bool tiled = g16_direct(A, lda, 0) && g16_direct(B, ldb, 0) && lda >= ((ca + 7) & ~7) && ldb >= ((cb + 7) & ~7);
   // (rows whose last vector is not whole may be followed by anything where rows run along the contraction: the few-row form then)
   const bool few = layout == 0 && M <= FEW_ROWS && (!tiled || (K & 7) || few16(M, N, K, p));
   if (!few && !tiled) {
-    set_error("hopmi_gemm16: operands need rows on 16 bytes that end on 16 bytes (hopmi_pad16)");
+    set_error("hopmi_gemm16: operands need rows on 16 bytes that end on 16 bytes, with strides up to 2^22 elements (hopmi_pad16)");
     return HOPMI_EINVAL;
   }
+  if (!few && p.splits == 0) { set_error("hopmi_gemm16: M=%d N=%d are more tiles than a launch counts", M, N); return HOPMI_EINVAL; }
   if (!few && p.splits > 1 && !ws) { set_error("hopmi_gemm16: null workspace"); return HOPMI_EINVAL; }
   hipStream_t st = static_cast<hipStream_t>(stream);
   auto go = [&](auto t) {

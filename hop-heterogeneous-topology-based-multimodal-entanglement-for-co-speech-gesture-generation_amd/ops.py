@@ -2437,8 +2437,8 @@ def linear_act(x, w, bias=None, residual=None, activation="none"):
 
     x (..., K), w (N, K), bias (N,) or None, residual broadcastable to (..., N) or None: all bf16 or all fp16 (under autocast all are cast
     to its type first; fp32 products are `linear`'s).  activation: "none", "relu", "gelu" (erf) or "silu".  Accumulation, bias,
-    activation and residual are fp32, with one rounding at the end.  Any sizes >= 1, strides and alignments; one to 64 rows take a form
-    that reads w once.  For the backward pass the values before the activation are kept in the operands' type, and dz = dy act'(z) is
+    activation and residual are fp32, with one rounding at the end.  Any sizes >= 1 (N and K up to 2^22), strides and alignments; few rows
+    take a form that reads w once.  For the backward pass the values before the activation are kept in the operands' type, and dz = dy act'(z) is
     rounded to it once, in front of the two products; the bias gradient sums the unrounded dz.  No atomics: the same bits every time.
     Differentiable once."""
     act = _ACT.get(activation)
@@ -2448,8 +2448,8 @@ def linear_act(x, w, bias=None, residual=None, activation="none"):
 
 
 class GradClip:
-    """The plan of a global-norm clip over a list of gradient tensors (hopmi_grad_clip), kept as an AdamPlan is: it holds the tensors and
-    their addresses; `clip_` launches at once.  tensors: fp32, bf16 or fp16 (mixed lists too) on one device, each filling its memory
+    """The plan of a global-norm clip over a list of gradient tensors (hopmi_grad_clip), kept as an AdamPlan is: it holds the tensor objects
+    (not the parameters: one whose .grad is replaced needs a new plan); `clip_` launches at once.  tensors: fp32, bf16 or fp16 (mixed lists too) on one device, each filling its memory
     without gaps, none of them sharing memory.  out: None = scale in place, or fp32 tensors of the same shapes and strides that receive
     the clipped values (what hopmi_adam_multi reads, from 16-bit gradients) while the gradients stay as they are."""
 

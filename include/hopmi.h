@@ -566,8 +566,8 @@ int hopmi_layernorm_bwd(const void* x, long long ldx, const void* dy, const floa
  * [M][ldr], z [M][ldz] nullable; z receives the values before the activation, rounded to dtype.  Operand rows have to start on 16 bytes
  * and to be backed by whole 16-byte vectors, with ZEROS behind a row's last element where rows run along the contraction
  * (hopmi_gemm16_direct says whether rows of `cols` elements are so by themselves; hopmi_pad16 copies rows into rows of ldp = a multiple
- * of 8 elements, zeros behind the N-th) -- except with layout 0 and M <= 64, which takes any alignment.
- * Operand strides up to 2^22 elements.  ws: hopmi_gemm16_ws_floats(M, N, K, layout) floats (contraction split over workgroups, added in
+ * of 8 elements, zeros behind the N-th), at strides of up to 2^22 elements -- except with layout 0 and M <= 64, which takes any
+ * alignment and stride.  ws: hopmi_gemm16_ws_floats(M, N, K, layout) floats (contraction split over workgroups, added in
  * split order by a second launch: bitwise reproducible). */
 size_t hopmi_gemm16_ws_floats(int M, int N, int K, int layout);
 int hopmi_gemm16_direct(const void* p, long long ld, int cols);

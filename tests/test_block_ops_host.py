@@ -62,12 +62,13 @@ def test_gemm16_entry_points_refuse():
     for kw in (dict(lda=63), dict(ldb=56), dict(ldc=127), dict(res=ONE, ldr=100)):
         assert call(**kw) == -1 and "stride" in _last(), kw
     assert call(lda=1 << 23) == -1 and "2^22" in _last()
+    assert call(M=(1 << 31) - 1, N=(1 << 31) - 1, ldc=1 << 31) == -1 and "more tiles" in _last()
     for kw in (dict(A=ctypes.c_void_p(18)), dict(lda=68), dict(lda=62, K=62), dict(ldb=128, ldc=128, N=122, lda=60, K=60, layout=1), dict(B=ctypes.c_void_p(24))):
         assert call(**kw) == -1 and "16 bytes" in _last(), kw
     assert L.hopmi_gemm16_ws_floats(128, 128, 4096, 0) > 0
     assert call(K=4096, lda=4096, ldb=4096, ws=None) == -1 and "workspace" in _last()
     assert L.hopmi_gemm16_ws_floats(16, 128, 768, 0) == 0 and L.hopmi_gemm16_ws_floats(0, 1, 1, 0) == 0
-    assert L.hopmi_gemm16_direct(ONE, 64, 64) == 1 and L.hopmi_gemm16_direct(ONE, 64, 60) == 0 and L.hopmi_gemm16_direct(ctypes.c_void_p(8), 64, 64) == 0
+    assert L.hopmi_gemm16_direct(ONE, 64, 64) == 1 and L.hopmi_gemm16_direct(ONE, 1 << 23, 64) == 0 and L.hopmi_gemm16_direct(ONE, 64, 60) == 0 and L.hopmi_gemm16_direct(ctypes.c_void_p(8), 64, 64) == 0
     assert L.hopmi_pad16(ONE, 5, ONE, 12, 4, 5, None) == -1 and L.hopmi_pad16(ONE, 5, ctypes.c_void_p(8), 8, 4, 5, None) == -1
     for kw in (dict(act=2, z=None), dict(ldz=12), dict(ws=None), dict(ldd=12), dict(dt=0)):
         a = dict(act=1, z=ONE, ldz=16, ws=ONE, ldd=16, dt=1)

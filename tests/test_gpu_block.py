@@ -631,3 +631,84 @@ def test_training_step_clips_by_max_grad_norm(recorded, monkeypatch):
     assert abs(after - 0.125 * norm) <= 1e-5 * norm
     assert not all(torch.equal(p, q) for p, q in zip(free.parameters(), clipped.parameters()))
 
+
+
+# --------------------------------------------------------------------------------------------------------- far offsets, wide strides
+def test_offsets_past_32_bits():
+    """Tensors of more than 2^31 elements: the last rows are as right as the first."""
+    t = torch.bfloat16
+    g = _rng(61)
+    D, M = 1024, (1 << 21) + 5
+    x = torch.zeros(M, D, device=_dev(), dtype=t)
+    w, b = (1 + 0.1 * _randn(g, D)).to(t), (0.1 * _randn(g, D)).to(t)
+    ends = torch.tensor([0, 1, M - 2, M - 1], device=_dev())
+    x[ends] = _randn(g, 4, D).to(t)
+    y = ops.layer_norm(x, w, b)
+    want = _ln_plain(x[ends].double(), w.double(), b.double(), 1e-5)[3]
+    check(y[ends], want, _half_step(t) * want.abs() + 1e-5 * (1 + want.abs()), "layer norm")        # 1e-5: 160 roundings of values of order one
+    assert torch.equal(y[2:-2], b.expand(M - 4, D))
+    del y
+    # the same rows through a product with as many results, and its input gradient
+    wl = (_randn(g, 1032, D) / 32).to(t)
+    xl = x.requires_grad_()
+    y = ops.linear_act(xl, wl)
+    want = x[ends].detach().double() @ wl.double().t()
+    check(y[ends], want, _half_step(t) * want.abs() + (D + 2) * 2 * U32 * (x[ends].detach().double().abs() @ wl.double().abs().t()) + _tiny(t), "linear")
+    dy = torch.zeros_like(y)
+    dy[ends] = _randn(g, 4, 1032).to(t)
+    del y
+    dx = torch.autograd.grad(ops.linear_act(xl, wl), xl, dy)[0]
+    want = dy[ends].double() @ wl.double()
+    check(dx[ends], want, _half_step(t) * want.abs() + 1034 * 2 * U32 * (dy[ends].double().abs() @ wl.double().abs()) + _tiny(t), "linear dx")
+    assert not dx[2:-2].any()
+    del dy, dx
+    flat = x.detach().view(-1)
+    flat.fill_(0.5)
+    n = ops.GradClip([flat[3:]]).clip_(1.0)
+    want = 0.5 * math.sqrt(M * D - 3)
+    assert abs(float(n) - want) <= 2 * U32 * want
+    v = 0.5 / (want + 1e-6)
+    assert (flat[:3] == 0.5).all() and (flat[3:].float() - v).abs().max() <= (_half_step(t) + 4 * U32) * v
+
+
+def test_wide_strides():
+    """Rows further apart than a tile's 32-bit offsets reach: read where they are by the few-row form, copied for the tiles."""
+    t = torch.float16
+    g = _rng(62)
+    ld = (1 << 22) + 24
+    buf = torch.zeros(70, ld, device=_dev(), dtype=t)
+    w = (_randn(g, 40, 96) / 10).to(t)
+    for M in (3, 70):
+        x = _randn(g, M, 96).to(t)
+        v = buf[:M, 8:104]
+        v.copy_(x)
+        assert torch.equal(ops.linear_act(v, w, activation="relu"), ops.linear_act(x, w, activation="relu"))
+        assert torch.equal(ops.layer_norm(v), ops.layer_norm(x))
+        a, c = v.detach().requires_grad_(), x.clone().requires_grad_()
+        dy = _randn(g, M, 40).to(t)
+        assert torch.equal(torch.autograd.grad(ops.linear_act(a, w), a, dy)[0], torch.autograd.grad(ops.linear_act(c, w), c, dy)[0])
+
+
+def test_grad_clip_plan_follows_its_tensors():
+    dev = _dev()
+    t, u = torch.full((1000,), 3.0, device=dev), torch.full((10, 10), 4.0, device=dev)
+    plan = ops.GradClip([t, u])
+    want = math.sqrt(9000 + 1600)
+    assert abs(float(plan.clip_(1e9)) - want) <= 2 * U32 * want
+    t.data = torch.full((1000,), 1.0, device=dev)                                # another piece of memory behind the same tensor
+    want = math.sqrt(1000 + 1600)
+    assert abs(float(plan.clip_(1.0)) - want) <= 2 * U32 * want and (t < 0.1).all() and (u < 0.1).all()
+    u.data = torch.zeros(3, device=dev)
+    with pytest.raises(_lib.HopmiError, match="any more"):
+        plan.clip_(1.0)
+    # two calls in flight on two streams, each with sums of its own
+    big = [torch.full((5_000_000,), float(k + 1), device=dev) for k in range(2)]
+    torch.cuda.synchronize()
+    norms = []
+    for k in range(2):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            norms.append(ops.GradClip([big[k]]).clip_(float("inf")))
+    torch.cuda.synchronize()
+    for k in range(2):
+        want = (k + 1) * math.sqrt(5_000_000)
+        assert abs(float(norms[k]) - want) <= 2 * U32 * want
