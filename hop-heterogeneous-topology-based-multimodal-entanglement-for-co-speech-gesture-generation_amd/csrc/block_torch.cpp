@@ -67,6 +67,12 @@ Tensor unwrap(const OptTensor& t) { return has(t) ? *t : Tensor(); }
 bool wants_grad(const OptTensor& t) { return has(t) && t->requires_grad(); }
 OptTensor dense(const OptTensor& t) { return has(t) && !t->is_contiguous() ? OptTensor(t->contiguous()) : t; }
 
+// What the kernels would not see: they read memory, and neither a tangent nor a pending negation is in it.
+void plain_values(const char* what, const OptTensor& t) {
+  if (!has(t)) return;
+  if (t->_fw_grad(0).defined()) refuse(what, ": no forward-mode derivative");
+  if (t->is_neg()) refuse(what, ": a tensor with a pending negation (.resolve_neg() makes a plain one)");
+}
 void on_device(const Tensor& first, const char* what) {
   if (!first.is_cuda()) refuse(what, ": the operand is on ", first.device(), "; this operator only runs on a ROCm device (no CPU fallback)");
 }
@@ -108,6 +114,8 @@ variable_list once(variable_list g, const variable_list& made_of) {
 }
 
 // ------------------------------------------------------------------------------------------------------------- layer norm
+constexpr int64_t MOST_WIDTH = int64_t(1) << 29;   // (a row's two sums, next to each other, count in 31 bits)
+
 int weight_code(const Tensor& x, const OptTensor& w, const OptTensor& b) { return code((has(w) ? *w : has(b) ? *b : x).scalar_type()); }
 
 Tensor ln_forward(const Tensor& x, const OptTensor& w, const OptTensor& b, double eps, Tensor* stat) {
@@ -166,7 +174,9 @@ Tensor layer_norm(const Tensor& x, const OptTensor& w0, const OptTensor& b0, dou
   const int64_t d = x.dim() > 0 ? x.size(-1) : 0;
   if (d < 1 || code(x.scalar_type()) < 0)
     refuse("layer_norm: x has shape ", x.sizes(), " and type ", x.scalar_type(), " (fp32, bf16 or fp16 with a last axis of at least 1)");
+  if (d > MOST_WIDTH) refuse("layer_norm: x has shape ", x.sizes(), ": a last axis of up to 2^29");
   if (!(eps >= 0.0)) refuse("layer_norm: eps=", eps);
+  for (const OptTensor& t : {OptTensor(x), w0, b0}) plain_values("layer_norm", t);
   on_device(x, "layer_norm");
   for (const auto& [name, t] : {std::pair<const char*, const OptTensor&>{"weight", w0}, {"bias", b0}}) {
     if (!has(t)) continue;
@@ -186,6 +196,7 @@ Tensor layer_norm(const Tensor& x, const OptTensor& w0, const OptTensor& b0, dou
 // ------------------------------------------------------------------------------------------------------------- linear_act
 constexpr int FEW_ROWS = 64;                       // up to here layout 0 takes operands of any alignment
 constexpr int64_t MOST = int64_t(1) << 22;         // longest row that the tiled products address
+constexpr int64_t MOST_ROWS = int64_t(1) << 30;
 
 bool direct(const Rows& r) { return L.hopmi_gemm16_direct(r.t.const_data_ptr(), r.ld, r.n) != 0; }
 // as hopmi_gemm16 takes it: as it lies where its rows start and end on 16 bytes, else copied into rows padded with zeros
@@ -292,6 +303,7 @@ struct LinearActFn : torch::autograd::Function<LinearActFn> {
 Tensor linear_act(const Tensor& x0, const Tensor& w0, const OptTensor& b0, const OptTensor& r0, int64_t act) {
   Tensor x = x0, w = w0;
   OptTensor b = b0, r = r0;
+  for (const OptTensor& t : {OptTensor(x), OptTensor(w), b, r}) plain_values("linear_act", t);
   if (at::autocast::is_autocast_enabled(at::kCUDA)) {
     const at::ScalarType t = at::autocast::get_autocast_dtype(at::kCUDA);
     x = x.to(t);
@@ -309,6 +321,7 @@ Tensor linear_act(const Tensor& x0, const Tensor& w0, const OptTensor& b0, const
   if (x.dim() < 1 || w.dim() != 2 || w.size(1) != x.size(-1) || w.size(0) < 1 || w.size(1) < 1)
     refuse("linear_act: x ", x.sizes(), " and w ", w.sizes(), " (N, K) do not fit, or have an empty side");
   if (w.size(0) > MOST || w.size(1) > MOST) refuse("linear_act: w ", w.sizes(), ": sides of up to 2^22");
+  if (x.numel() / x.size(-1) > MOST_ROWS) refuse("linear_act: x has shape ", x.sizes(), ": up to 2^30 rows");
   if (has(b) && (b->dim() != 1 || b->size(0) != w.size(0))) refuse("linear_act: bias has shape ", b->sizes(), ", w ", w.sizes());
   if (has(r)) {
     at::DimVector shape(x.sizes().begin(), x.sizes().end());
@@ -332,52 +345,77 @@ bool fills(const Tensor& t) { return t.is_contiguous() || t.is_non_overlapping_a
 
 struct ClipPlan {
   std::vector<Tensor> in, to;
-  mutable std::vector<const void*> src;              // (addresses are read again by every call)
-  mutable std::vector<void*> dst;
+  std::vector<const void*> src;
+  std::vector<void*> dst;
   std::vector<long long> n;
   std::vector<int> dt;
-  bool into = false;
+  bool into = false, separate = false;               // separate: apart() has seen these addresses
 
   ClipPlan(std::vector<Tensor> tensors, std::optional<std::vector<Tensor>> outs) : in(std::move(tensors)), into(outs.has_value()) {
     if (outs) to = std::move(*outs);
     if (in.empty()) refuse("GradClip: an empty list of tensors");
     if (into && to.size() != in.size()) refuse("GradClip: ", to.size(), " outputs for ", in.size(), " tensors");
     on_device(in[0], "GradClip");
-    struct Span { uintptr_t p, end; const char* list; size_t i; };
-    std::vector<Span> spans;
+    src.resize(in.size());
+    dst.resize(into ? in.size() : 0);
+    n.resize(in.size());
+    dt.resize(in.size());
+    read(true);
+    apart();
+  }
+
+  // The tensors' memory as it is now (`.data = ...` changes it under a plan), checked again.
+  void read(bool first) {
+    const at::Device dev = in[0].device();
+    if (!dev.is_cuda()) refuse("GradClip: tensors[0] is on ", dev);
     for (size_t i = 0; i < in.size(); ++i) {
       const Tensor& t = in[i];
-      if (t.device() != in[0].device()) refuse("GradClip: tensors[", i, "] is on ", t.device(), ", the first on ", in[0].device());
+      if (t.device() != dev) refuse("GradClip: tensors[", i, "] is on ", t.device(), ", the first on ", dev);
       if (t.layout() != at::kStrided || code(t.scalar_type()) < 0 || !fills(t))
         refuse("GradClip: tensors[", i, "] (", t.scalar_type(), ", shape ", t.sizes(), ") is not an fp32, bf16 or fp16 tensor without gaps "
                "(.contiguous() makes one)");
-      src.push_back(t.const_data_ptr());
-      n.push_back(t.numel());
-      dt.push_back(code(t.scalar_type()));
-      if (t.numel() > 0) spans.push_back({reinterpret_cast<uintptr_t>(t.const_data_ptr()), 0, "tensors", i}), spans.back().end = spans.back().p + t.numel() * t.element_size();
+      if (t.is_neg()) refuse("GradClip: tensors[", i, "] has a pending negation (.resolve_neg() makes a plain tensor)");
+      const void* p = t.const_data_ptr();
+      const int c = code(t.scalar_type());
+      if (!first && (n[i] != t.numel() || dt[i] != c)) refuse("GradClip: tensors[", i, "] is not the tensor that the plan was made for any more");
+      if (p != src[i]) separate = false;
+      src[i] = p;
+      n[i] = t.numel();
+      dt[i] = c;
       if (!into) continue;
       const Tensor& o = to[i];
-      if (o.device() != in[0].device()) refuse("GradClip: out[", i, "] is on ", o.device(), ", the first tensor on ", in[0].device());
-      if (o.layout() != at::kStrided || o.scalar_type() != at::kFloat || o.sizes() != t.sizes() || !fills(o) ||
+      if (o.device() != dev) refuse("GradClip: out[", i, "] is on ", o.device(), ", the first tensor on ", dev);
+      if (o.layout() != at::kStrided || o.scalar_type() != at::kFloat || o.sizes() != t.sizes() || !fills(o) || o.is_neg() ||
           (!(t.is_contiguous() && o.is_contiguous()) && o.strides() != t.strides()))
         refuse("GradClip: out[", i, "] is not an fp32 tensor of tensors[", i, "]'s shape and strides");
-      dst.push_back(o.mutable_data_ptr());
-      if (o.numel() > 0) spans.push_back({reinterpret_cast<uintptr_t>(o.const_data_ptr()), 0, "out", i}), spans.back().end = spans.back().p + o.numel() * 4;
+      void* q = o.mutable_data_ptr();
+      if (q != dst[i]) separate = false;
+      dst[i] = q;
+    }
+  }
+
+  void apart() {
+    struct Span { uintptr_t p, end; const char* list; size_t i; };
+    std::vector<Span> spans;
+    for (size_t i = 0; i < in.size(); ++i) {
+      if (n[i] == 0) continue;
+      const auto p = reinterpret_cast<uintptr_t>(src[i]);
+      spans.push_back({p, p + n[i] * in[i].element_size(), "tensors", i});
+      if (!into) continue;
+      const auto q = reinterpret_cast<uintptr_t>(dst[i]);
+      spans.push_back({q, q + n[i] * 4, "out", i});
     }
     std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.p < b.p; });
     for (size_t k = 1; k < spans.size(); ++k)
       if (spans[k - 1].end > spans[k].p)
         refuse("GradClip: ", spans[k - 1].list, "[", spans[k - 1].i, "] and ", spans[k].list, "[", spans[k].i, "] share memory");
+    separate = true;
   }
 
-  Tensor clip(double max_norm) const {
+  Tensor clip(double max_norm) {
     if (!(max_norm >= 0.0)) refuse("GradClip: max_norm=", max_norm);
-    for (size_t i = 0; i < in.size(); ++i) {
-      if (in[i].numel() != n[i] || code(in[i].scalar_type()) != dt[i] || (into && to[i].numel() != n[i]))
-        refuse("GradClip: tensors[", i, "] is not the tensor that the plan was made for any more");
-      src[i] = in[i].const_data_ptr();
-      if (into) dst[i] = to[i].mutable_data_ptr();
-    }
+    read(false);
+    if (!separate) apart();
     const c10::DeviceGuard guard(in[0].device());
     at::NoGradGuard no_grad;
     const auto opt = at::TensorOptions().device(in[0].device());

@@ -347,6 +347,8 @@ __global__ __launch_bounds__(1024) void ln_reduce_kernel(const float* __restrict
   }
 }
 
+constexpr int LN_WIDEST = 1 << 29;                           // (2 D and what is added to it count in 31 bits)
+
 // which form a row width takes, by its number of 16-byte vectors: a wave up to 256, then two vectors per thread
 static int ln_form(int D, int dtype) {
   const int vecs = D / (dtype == T_F32 ? 4 : 8);
@@ -392,8 +394,8 @@ static void ln_bwd_go(const void* x, long long ldx, const void* dy, const float*
                       float* part, int M, int D, int grid, hipStream_t st) {
   const auto k = ln_bwd_kernel<T, WT, NV, TPR>;
   const size_t lds = TPR == 64 && part != nullptr ? 8 * D * sizeof(float) : 0;               // up to 66 KB
-  static const hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, 72 * 1024);
-  (void)once;
+  static std::atomic<unsigned long long> told{0};
+  allow_lds(reinterpret_cast<const void*>(k), 72 * 1024, told);
   hipLaunchKernelGGL(k, dim3(grid), dim3(TPR == 64 ? 256 : TPR), lds, st, static_cast<const T*>(x), ldx,
                      static_cast<const T*>(dy), mean, rstd, static_cast<const WT*>(w), static_cast<T*>(dx), part, M, D);
 }
@@ -423,7 +425,7 @@ static int ln_check(const char* what, int dtype, int wdtype, int M, int D, long 
     set_error("%s: dtype=%d, weights %d (0 fp32, 1 bf16, 2 fp16; weights of the same type or fp32)", what, dtype, wdtype);
     return HOPMI_EINVAL;
   }
-  if (M < 1 || D < 1 || ldx < D) { set_error("%s: bad sizes M=%d D=%d ldx=%lld", what, M, D, ldx); return HOPMI_EINVAL; }
+  if (M < 1 || D < 1 || D > LN_WIDEST || ldx < D) { set_error("%s: bad sizes M=%d D=%d ldx=%lld", what, M, D, ldx); return HOPMI_EINVAL; }
   return HOPMI_OK;
 }
 
@@ -453,7 +455,7 @@ extern "C" int hopmi_layernorm_fwd(const void* x, long long ldx, const void* wei
 }
 
 extern "C" size_t hopmi_layernorm_bwd_ws_floats(int M, int D, int dtype) {
-  if (M < 1 || D < 1 || dtype < T_F32 || dtype > T_F16) return 0;
+  if (M < 1 || D < 1 || D > LN_WIDEST || dtype < T_F32 || dtype > T_F16) return 0;
   return (size_t)ln_bwd_grid(M, D, dtype) * 2 * D;
 }
 

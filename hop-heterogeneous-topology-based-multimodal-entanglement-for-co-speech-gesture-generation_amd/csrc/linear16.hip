@@ -704,8 +704,8 @@ static bool few16(int M, int N, int K, const Plan16& p) {
 template <typename T, int BM, int BN, int WR, int WC, int ST, bool KA, bool KB> static void gemm16_go(const Gemm16<T>& G, hipStream_t st) {
   constexpr int bytes = ST * (BM + BN) * G16_BK * 2;
   const auto k = gemm16_kernel<T, BM, BN, WR, WC, ST, KA, KB>;
-  static const hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  (void)once;
+  static std::atomic<unsigned long long> told{0};
+  allow_lds(reinterpret_cast<const void*>(k), bytes, told);
   hipLaunchKernelGGL(k, dim3((unsigned)(G.tiles_m * G.tiles_n * G.splits)), dim3(64 * WR * WC), bytes, st, G);
 }
 template <typename T> static void gemm16_run(Gemm16<T> G, int layout, bool few, const Plan16& p, float* ws, hipStream_t st) {
@@ -742,6 +742,11 @@ template <typename T> static void gemm16_run(Gemm16<T> G, int layout, bool few, 
 static bool g16_direct(const void* p, long long ld, int cols) {
   return !((reinterpret_cast<uintptr_t>(p) & 15) | (ld & 7) | (cols & 7)) && ld <= 1 << 22;
 }
+// sides whose sums with a tile's count in 31 bits
+static bool g16_sides(int M, int N, int K) {
+  constexpr int MOST = 1 << 30;
+  return M >= 1 && N >= 1 && K >= 1 && M <= MOST && N <= MOST && K <= MOST;
+}
 static int act_bwd_groups(int M, int N) {
   const int strips = (N + 511) / 512;
   const long long quads = ((long long)M + 3) / 4;
@@ -755,7 +760,7 @@ static int act_bwd_groups(int M, int N) {
 using namespace hopmi;
 
 extern "C" size_t hopmi_gemm16_ws_floats(int M, int N, int K, int layout) {
-  if (M < 1 || N < 1 || K < 1 || layout < 0 || layout > 2) return 0;
+  if (!g16_sides(M, N, K) || layout < 0 || layout > 2) return 0;
   const Plan16 p = plan16(M, N, K, layout);
   if (layout == 0 && M <= FEW_ROWS && few16(M, N, K, p)) return 0;
   return p.splits > 1 ? (size_t)p.splits * M * N : 0;
@@ -771,6 +776,7 @@ extern "C" int hopmi_gemm16(const void* A, long long lda, const void* B, long lo
     set_error("hopmi_gemm16: M=%d N=%d K=%d layout=%d activation=%d", M, N, K, layout, act);
     return HOPMI_EINVAL;
   }
+  if (!g16_sides(M, N, K)) { set_error("hopmi_gemm16: M=%d N=%d K=%d (sides of up to 2^30) are more tiles than a launch counts", M, N, K); return HOPMI_EINVAL; }
   if (dtype != T_BF16 && dtype != T_F16) { set_error("hopmi_gemm16: dtype=%d (1 bf16, 2 fp16)", dtype); return HOPMI_EINVAL; }
   const int ca = layout == 2 ? M : K, cb = layout == 0 ? K : N;
   if (lda < ca || ldb < cb || ldc < N || (res && ldr < N) || (z && ldz < N)) { set_error("hopmi_gemm16: a row stride below the row's length"); return HOPMI_EINVAL; }
@@ -810,11 +816,11 @@ extern "C" int hopmi_pad16(const void* src, long long lds_, void* dst, long long
   return check_launch("hopmi_pad16");
 }
 
-extern "C" size_t hopmi_act_bwd16_ws_floats(int M, int N) { return M < 1 || N < 1 ? 0 : (size_t)act_bwd_groups(M, N) * N; }
+extern "C" size_t hopmi_act_bwd16_ws_floats(int M, int N) { return !g16_sides(M, N, 1) ? 0 : (size_t)act_bwd_groups(M, N) * N; }
 
 extern "C" int hopmi_act_bwd16(const void* dy, long long ldy, const void* z, long long ldz, void* dz, long long ldd, void* dbias, float* ws,
                                int act, int M, int N, int dtype, void* stream) {
-  if (!dy || M < 1 || N < 1 || ldy < N || act < ACT_NONE || act > ACT_SILU || (dtype != T_BF16 && dtype != T_F16) || (act != ACT_NONE && !z) ||
+  if (!dy || !g16_sides(M, N, 1) || ldy < N || act < ACT_NONE || act > ACT_SILU || (dtype != T_BF16 && dtype != T_F16) || (act != ACT_NONE && !z) ||
       (z && ldz < ((N + 7) & ~7)) || (dz && (ldd < N || (ldd & 7))) || (dbias && !ws)) {
     set_error("hopmi_act_bwd16: M=%d N=%d activation=%d dtype=%d, a bad stride, or a null pointer", M, N, act, dtype);
     return HOPMI_EINVAL;

@@ -4,6 +4,8 @@
 #pragma once
 #include "common.h"
 
+#include <atomic>
+
 namespace hopmi {
 
 constexpr int T_F32 = 0, T_BF16 = 1, T_F16 = 2;      // dtype codes of the C ABI
@@ -44,6 +46,16 @@ __device__ __forceinline__ u32x4_t vpack(const float* f, const float*) {
 }
 template <typename T> __device__ __forceinline__ u32x4_t vpack(const float* f, const T* t) {
   return u32x4_t{pk2(f[0], f[1], t), pk2(f[2], f[3], t), pk2(f[4], f[5], t), pk2(f[6], f[7], t)};
+}
+
+// Lets a kernel have `bytes` of dynamic LDS on the current device; `done` (one per kernel) holds the devices that have been told.
+inline void allow_lds(const void* kernel, int bytes, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess) return;              // (the launch reports it)
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_relaxed) & bit) return;
+  if (hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  else (void)hipGetLastError();
 }
 
 template <typename T> __device__ __forceinline__ float to_f(T v) { return (float)v; }

@@ -109,3 +109,34 @@ def test_recorded_step_over_ranks_refuses_max_grad_norm(tmp_path):
         assert hopmi.GraphedTrainStep(types.SimpleNamespace(), mod, mod, None, None, force_exchange=True).exchange
     finally:
         dist.destroy_process_group()
+
+
+def test_sizes_that_indices_do_not_count_are_refused():
+    L = _lib.lib()
+    big, most = (1 << 31) - 1, 1 << 30
+    assert L.hopmi_layernorm_fwd(ONE, big, ONE, ONE, 0, ONE, None, None, 4, most, 1e-5, 0, None) == -1 and "sizes" in _last()
+    assert L.hopmi_layernorm_bwd(ONE, big, ONE, ONE, ONE, ONE, 0, ONE, ONE, ONE, ONE, 4, most, 0, None) == -1 and "sizes" in _last()
+    assert L.hopmi_layernorm_bwd_ws_floats(4, most, 0) == 0 and L.hopmi_layernorm_bwd_ws_floats(4, 1 << 29, 0) == 1 << 32
+    gemm = lambda M, N, K, layout: L.hopmi_gemm16(ONE, 1 << 32, ONE, 1 << 32, layout, ONE, 1 << 32, None, None, 0, None, 0, 0, M, N, K, 1, ONE, None)
+    for layout in range(3):
+        for side in ((most + 1, 8, 8), (8, most + 1, 8), (8, 8, most + 1), (4, 8, big)):
+            assert gemm(*side, layout) == -1 and "2^30" in _last(), (side, layout)
+            assert L.hopmi_gemm16_ws_floats(*side, layout) == 0
+    assert L.hopmi_act_bwd16(ONE, 1 << 32, ONE, 1 << 32, ONE, 1 << 32, ONE, ONE, 1, 4, most + 1, 1, None) == -1
+    assert L.hopmi_act_bwd16_ws_floats(4, most + 1) == 0
+
+
+def test_tangents_and_pending_negations_are_refused():
+    """The kernels read memory: a forward-mode tangent would be lost, a pending negation not applied."""
+    import torch.autograd.forward_ad as fwad
+    x, w = torch.zeros(4, 8), torch.zeros(8, 8)
+    with fwad.dual_level():
+        d = fwad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: ops.layer_norm(d), lambda: ops.layer_norm(x, d[0]), lambda: ops.linear_act(d, w), lambda: ops.linear_act(x, w, None, d)):
+            with pytest.raises(_lib.HopmiError, match="forward-mode"):
+                call()
+    n = torch.complex(x, x).conj().imag
+    assert n.is_neg()
+    for call in (lambda: ops.layer_norm(n), lambda: ops.linear_act(n, w), lambda: ops.linear_act(x, w, n[0])):
+        with pytest.raises(_lib.HopmiError, match="negation"):
+            call()

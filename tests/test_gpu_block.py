@@ -712,3 +712,29 @@ def test_grad_clip_plan_follows_its_tensors():
     for k in range(2):
         want = (k + 1) * math.sqrt(5_000_000)
         assert abs(float(norms[k]) - want) <= 2 * U32 * want
+
+
+def test_grad_clip_plan_looks_at_moved_tensors_again():
+    """Memory behind a plan's tensors may be exchanged: what the plan refused at first it refuses then too, before any launch."""
+    dev = _dev()
+    t, u, o = torch.ones(1000, device=dev), torch.ones(1000, device=dev), torch.zeros(1000, device=dev)
+    plan, into = ops.GradClip([t, u]), ops.GradClip([u], out=[o])
+    both = torch.full((1500,), 2.0, device=dev)
+    keep = u.data
+    t.data, u.data = both[:1000], both[500:]
+    for _ in range(2):                                       # (not only the first time)
+        with pytest.raises(_lib.HopmiError, match="share memory"):
+            plan.clip_(1.0)
+    u.data = torch.ones(2000, device=dev)[::2]
+    with pytest.raises(_lib.HopmiError, match="without gaps"):
+        plan.clip_(1.0)
+    u.data = torch.ones(1000)
+    for p in (plan, into):
+        with pytest.raises(_lib.HopmiError, match="is on cpu"):
+            p.clip_(1.0)
+    u.data, o.data = keep, torch.zeros(999, device=dev)
+    with pytest.raises(_lib.HopmiError, match="shape"):
+        into.clip_(1.0)
+    want = math.sqrt(1000 * 4 + 1000)
+    assert abs(float(plan.clip_(1e9)) - want) <= 2 * U32 * want
+    assert (both == 2).all() and (u == 1).all()
