@@ -3,12 +3,12 @@
 //   mu = sum_d x / D      v = sum_d (x - mu)^2 / D      r = 1 / sqrt(v + eps)      xh = (x - mu) r      y = xh g + b
 //   dx = r (g dy - mean_d(g dy) - xh mean_d(g dy xh))       dg = sum_rows dy xh       db = sum_rows dy
 //
-// Bound: HBM (8 / 22 operations per element against 4-8 / 6-12 bytes); measured, in a recorded graph: forward 8192 x 4096 fp32 41.8 us (6.5 TB/s
-// of x and y together, some of it from the 256 MB cache), backward 85.6 (4.7 TB/s of x, dy, dx); 32768 x 1024 bf16 22.4 and 41.0; a large copy
-// moves 5.2 TB/s.  Below some 10 MB the launches bound it: 4352 x 768 bf16 5.0 and 12.9 us (two launches), one window of 34 rows 3.0.  So each pass reads x (and dy) once: a row stays in the
-// registers of one wave (up to 256 16-byte vectors) or of a workgroup of 256 (up to 512), 512 (1024) or 1024 threads (2048);
-// wider rows are re-read (from the caches) by the looped form.  The variance is taken around the mean, not as E x^2 - mu^2: the row
-// is in registers, a second pass over it costs no memory.
+// Bound: HBM (8 / 22 operations per element against 4-8 / 6-12 bytes); measured, in a recorded graph: forward 8192 x 4096 fp32 41.8 us
+// (6.5 TB/s of x and y together, some of it from the 256 MB cache), backward 85.6 (4.7 TB/s of x, dy, dx); 32768 x 1024 bf16 22.4 and
+// 41.0; a large copy moves 5.2 TB/s.  Below some 10 MB the launches bound it: 4352 x 768 bf16 5.0 and 12.9 us (two launches), one window
+// of 34 rows 3.0.  So each pass reads x (and dy) once: a row stays in the registers of one wave (up to 256 16-byte vectors) or of a
+// workgroup of 256 (up to 512), 512 (1024) or 1024 threads (2048); wider rows are re-read (from the caches) by the looped form.
+// The variance is taken around the mean, not as E x^2 - mu^2: the row is in registers, a second pass over it costs no memory.
 // The weights' gradients are sums over the rows: a workgroup walks rows blockIdx, blockIdx + grid, ... and keeps its columns' sums in
 // registers, leaves one partial row [2][D] in the workspace, and a second launch adds the partial rows in index order (no atomics:
 // the same bits every time).

@@ -10,14 +10,22 @@
 // between) in the order in which it lies in memory, and read as MFMA fragments either straight (contraction-contiguous: ds_read_b128)
 // or through the transposing LDS read (ds_read_b64_tr_b16), so no operand is ever transposed in memory.
 // v_mfma_f32_16x16x32: lane 16 q + n holds A[n][8 q ..], B[8 q ..][n] and D[4 q + r][n].  The result's COLUMNS are put on D's rows, so a
-// lane ends with four consecutive columns of one row and every epilogue access is 8 bytes.
+// lane ends with four consecutive columns of one row (a 16-byte LDS write); through LDS every thread then gets eight columns of a row,
+// and every access of the epilogue is 16 bytes.
 // LDS images are swizzled through the SOURCE address of each lane's 16 bytes (the DMA's LDS side is fixed: lane l at base + 16 l):
 //   contraction-contiguous tile [rows][64]: 128-byte rows, 16-byte chunk c at c ^ ((row >> 1) & 7): the sixteen lanes that a 16-byte read serves
 //   together (0-3, 12-15, 20-23, 24-27, ...) lie on sixteen different slots
 //   result-contiguous tile [64][cols]: mn_swizzle() below: the eight rows that one half wave reads lie on eight different 32-byte groups
 // Edges: rows past the end are clamped to the last one (their results are not stored); contraction indices past the end read 16 bytes
 // of zeros instead, on both operands.  Operands whose rows do not start on 16 bytes, or end inside one, are copied once into rows
-// padded with zeros.
+// padded with zeros (2171 x 1021 fp16: 5.2 us).
+// Bound: the matrix cores for large products, launch, first loads and the epilogue's bytes for small ones.  Measured, bf16, us (2 M N K
+// over the time; the same product of the BLAS library on the same card; a product of 8192^3 runs there at 1590 TFLOP/s):
+//   16384 x 4096 x 4096   x w^T 405 (1357 TFLOP/s; library 365)   dX 408 (1347; 420)   dW 405 (1357; 470)
+//   4352 x 768 -> 2304    x w^T 24.1 (640; 26.8)                   dX 22.9 (672; 25.4)  dW 29.9 (515; 36.3)
+//   one row, 768 -> 2304  3.6 (few-row form: 3.5 MB of W)          34 rows, 768 -> 768 with bias and residual 6.0
+// With bias, gelu, residual and the kept pre-activation (three more streams of the result's size) 16384 x 4096 x 4096 takes 470-490,
+// 4352 x 768 -> 2304 32.
 #include "t16_dev.h"
 
 #include <type_traits>
@@ -41,7 +49,7 @@ __device__ __forceinline__ f32x4 mfma16x32(u32x4_t a, u32x4_t b, f32x4 c, const 
 // a smooth function that a polynomial in t without constant term (Q -> 0 with t) meets to 5e-6 of its value on 0 <= u <= 14 (least
 // largest relative error, fitted against 64-bit values); beyond, exp(-u^2 / 2) is 0 in fp32.  RELATIVE accuracy far below the result's
 // rounding (2^-9 / 2^-12) also in the tail.  The epilogue of a product with a short contraction is bound by these instructions (15 per
-// gelu, two of them at a quarter of the rate; erff alone takes twice that).
+// gelu, two of them at a quarter of the rate).
 __device__ __forceinline__ float gauss_tail(float u, float e) {      // e = exp(-u^2 / 2)
   const float t = __builtin_amdgcn_rcpf(fmaf(0.31f, u, 1.f));
   float q = fmaf(-0.07392919063568115f, t, 0.18044988811016083f);
@@ -557,7 +565,9 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void gemm16_few_kernel(Gemm16<T> G)
 }
 
 // dz = dY act'(z) (rows padded with zeros to ldd, a multiple of 8; null: not wanted) and the partial column sums of the UNROUNDED dz of
-// each row group, part [gridDim.y][N] (null: not wanted).  A wave takes 512 columns of every fourth row of its group.
+// each row group, part [gridDim.y][N] (null: not wanted).  A wave takes 512 columns of every fourth row of its group.  Bound: HBM (two
+// reads, one write): 16384 x 4096 bf16 gelu 83-87 us (4.7 TB/s), 4352 x 2304 16.7 (3.6 TB/s: five rows per wave do not hide the first's
+// latency).
 template <typename T>
 __global__ __launch_bounds__(256) void act_bwd16_kernel(const T* __restrict__ dy, long long ldy, const T* __restrict__ z, long long ldz,
                                                         T* __restrict__ dz, long long ldd, float* __restrict__ part, int M, int N, int act) {
