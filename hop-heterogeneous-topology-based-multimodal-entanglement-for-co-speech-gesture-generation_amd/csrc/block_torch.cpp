@@ -35,7 +35,8 @@ PyObject* g_error = nullptr;                       // _lib.HopmiError
 
 #define HOPMI_API(X)                                                                                                       \
   X(hopmi_last_error) X(hopmi_layernorm_fwd) X(hopmi_layernorm_bwd_ws_floats) X(hopmi_layernorm_bwd) X(hopmi_gemm16_ws_floats) \
-  X(hopmi_gemm16) X(hopmi_gemm16_direct) X(hopmi_pad16) X(hopmi_act_bwd16_ws_floats) X(hopmi_act_bwd16) X(hopmi_grad_clip_ws_bytes) X(hopmi_grad_clip)
+  X(hopmi_gemm16) X(hopmi_gemm16_direct) X(hopmi_pad16) X(hopmi_pad16_two) X(hopmi_act_bwd16_ws_floats) X(hopmi_act_bwd16) \
+  X(hopmi_linear16_bwd_ws_floats) X(hopmi_linear16_bwd) X(hopmi_grad_clip_ws_bytes) X(hopmi_grad_clip)
 struct Api {
 #define X(f) decltype(&::f) f = nullptr;
   HOPMI_API(X)
@@ -200,12 +201,27 @@ constexpr int64_t MOST_ROWS = int64_t(1) << 30;
 
 bool direct(const Rows& r) { return L.hopmi_gemm16_direct(r.t.const_data_ptr(), r.ld, r.n) != 0; }
 // as hopmi_gemm16 takes it: as it lies where its rows start and end on 16 bytes, else copied into rows padded with zeros
+Rows padding(const Rows& r) {
+  const int64_t ld = (int64_t(r.n) + 7) / 8 * 8;
+  return Rows{at::empty({r.m, ld}, r.t.options()), ld, r.m, r.n};
+}
 Rows operand(const Rows& r) {
   if (direct(r)) return r;
-  const int64_t ld = (int64_t(r.n) + 7) / 8 * 8;
-  Rows p{at::empty({r.m, ld}, r.t.options()), ld, r.m, r.n};
-  check(L.hopmi_pad16(r.t.const_data_ptr(), r.ld, out(p.t), ld, r.m, r.n, stream(r.t)), "hopmi_pad16");
+  Rows p = padding(r);
+  check(L.hopmi_pad16(r.t.const_data_ptr(), r.ld, out(p.t), p.ld, r.m, r.n, stream(r.t)), "hopmi_pad16");
   return p;
+}
+void operands(Rows& a, Rows& b) {
+  if (direct(a) || direct(b)) {
+    a = operand(a);
+    b = operand(b);
+    return;
+  }
+  Rows p = padding(a), q = padding(b);
+  check(L.hopmi_pad16_two(a.t.const_data_ptr(), a.ld, out(p.t), p.ld, a.m, a.n, b.t.const_data_ptr(), b.ld, out(q.t), q.ld, b.m, b.n, stream(a.t)),
+        "hopmi_pad16_two");
+  a = std::move(p);
+  b = std::move(q);
 }
 
 void gemm(const Rows& a, const Rows& b, int layout, const Tensor& c, int M, int N, int K, const OptTensor& bias, const Rows& res, const Tensor& z,
@@ -231,8 +247,7 @@ Linear16 linear_forward(const Tensor& x, const Tensor& w, const OptTensor& bias,
   if (M == 0) return o;
   const Rows r = has(res) ? rows(*res, N) : Rows{};
   if (M > FEW_ROWS) {
-    o.x = operand(o.x);
-    o.w = operand(o.w);
+    operands(o.x, o.w);
   }
   gemm(o.x, o.w, 0, o.y, M, N, K, bias, r, o.z, act);
   return o;
@@ -278,21 +293,31 @@ struct LinearActFn : torch::autograd::Function<LinearActFn> {
           dz.t = at::empty({M, dz.ld}, x.options());
         }
         const bool make = dz.t.unsafeGetTensorImpl() != d.t.unsafeGetTensorImpl();
+        const bool both = need_x && need_w;        // (with the bias gradient's last sums in the same launch)
+        Tensor ws;
         if (make || need_b) {
-          Tensor ws;
           if (need_b) ws = at::empty({(int64_t)L.hopmi_act_bwd16_ws_floats(M, (int)N)}, x.options().dtype(at::kFloat));
-          check(L.hopmi_act_bwd16(d.t.const_data_ptr(), d.ld, ptr(z), z.defined() ? z.size(1) : 0, make ? out(dz.t) : nullptr, dz.ld, out(g[2]),
-                                  fout(ws), act, M, (int)N, code(x.scalar_type()), stream(x)), "hopmi_act_bwd16");
+          check(L.hopmi_act_bwd16(d.t.const_data_ptr(), d.ld, ptr(z), z.defined() ? z.size(1) : 0, make ? out(dz.t) : nullptr, dz.ld,
+                                  both ? nullptr : out(g[2]), fout(ws), act, M, (int)N, code(x.scalar_type()), stream(x)), "hopmi_act_bwd16");
         }
-        auto padded = [](const Tensor& p, const Tensor& t) {
+        auto kept = [](const Tensor& p, const Tensor& t) {          // (the forward's padded copy, if there is one)
           Rows r = rows(t, t.size(-1));
-          if (!p.defined()) return operand(r);
+          if (!p.defined()) return r;
           r.t = p;
           r.ld = p.size(1);
+          r.n = (int)p.size(1);
           return r;
         };
-        if (need_x) gemm(dz, padded(s[4], w), 1, g[0], M, (int)K, (int)N, OptTensor(), Rows{}, Tensor(), 0);
-        if (need_w) gemm(dz, padded(s[3], x), 2, g[1], (int)N, (int)K, M, OptTensor(), Rows{}, Tensor(), 0);
+        if (both) {
+          Rows pw = kept(s[4], w), px = kept(s[3], x);
+          operands(pw, px);
+          const size_t n = L.hopmi_linear16_bwd_ws_floats(M, (int)N, (int)K);
+          Tensor ws2;
+          if (n > 0) ws2 = at::empty({(int64_t)n}, x.options().dtype(at::kFloat));
+          check(L.hopmi_linear16_bwd(dz.t.const_data_ptr(), dz.ld, pw.t.const_data_ptr(), pw.ld, px.t.const_data_ptr(), px.ld, out(g[0]), out(g[1]),
+                                     fout(ws), out(g[2]), M, (int)N, (int)K, code(x.scalar_type()), fout(ws2), stream(x)), "hopmi_linear16_bwd");
+        } else if (need_x) gemm(dz, operand(kept(s[4], w)), 1, g[0], M, (int)K, (int)N, OptTensor(), Rows{}, Tensor(), 0);
+        else if (need_w) gemm(dz, operand(kept(s[3], x)), 2, g[1], (int)N, (int)K, M, OptTensor(), Rows{}, Tensor(), 0);
       }
       if (need_r) g[3] = dy;
     }

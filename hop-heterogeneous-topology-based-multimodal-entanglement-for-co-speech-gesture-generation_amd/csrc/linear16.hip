@@ -18,7 +18,7 @@
 //   result-contiguous tile [64][cols]: mn_swizzle() below: the eight rows that one half wave reads lie on eight different 32-byte groups
 // Edges: rows past the end are clamped to the last one (their results are not stored); contraction indices past the end read 16 bytes
 // of zeros instead, on both operands.  Operands whose rows do not start on 16 bytes, or end inside one, are copied once into rows
-// padded with zeros (2171 x 1021 fp16: 5.2 us).
+// padded with zeros, both in one launch (2171 x 1021 and 427 x 1021 fp16: 6.2 us).
 // Bound: the matrix cores for large products, launch, first loads and the epilogue's bytes for small ones.  Measured, bf16, us (2 M N K
 // over the time; the same product of the BLAS library on the same card; a product of 8192^3 runs there at 1590 TFLOP/s):
 //   16384 x 4096 x 4096   x w^T 405 (1357 TFLOP/s; library 365)   dX 408 (1347; 420)   dW 405 (1357; 470)
@@ -28,6 +28,7 @@
 // 4352 x 768 -> 2304 32.
 #include "t16_dev.h"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace hopmi {
@@ -269,18 +270,16 @@ template <int N> __device__ __forceinline__ void wait_and_meet() {
 // step, between its halves: there, every wave has read all of this step (its buffer takes step s + ST) and step s + 1 has landed (the
 // younger DMA stays in flight: counted).
 template <typename T, int BM, int BN, int WR, int WC, int ST, bool KA, bool KB>
-__global__ __launch_bounds__(64 * WR * WC, 2) void gemm16_kernel(Gemm16<T> G) {
+__device__ __forceinline__ void gemm16_tile(const Gemm16<T>& G, int id, char* lds) {
   constexpr int NW = WR * WC, RB = BM / WR / 16, CB = BN / WC / 16, BK = G16_BK;
   using TA = Tile16<T, BM, NW, KA>;
   using TB = Tile16<T, BN, NW, KB>;
   constexpr int SB = TA::BYTES + TB::BYTES, NI = TA::NI + TB::NI;
-  extern __shared__ __attribute__((aligned(1024))) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, q = lane >> 4;
   const int wr = wave / WC, wc = wave % WC;
   // workgroups go to the eight XCDs in turn: give each XCD one contiguous stretch of the tile order, and walk that order in groups of
   // eight tile rows, so that what an L2 holds is used by its own workgroups
   const int tiles = G.tiles_m * G.tiles_n, total = tiles * G.splits;
-  int id = blockIdx.x;
   {
     const int per = total / 8, rem = total % 8, x = id % 8, i = id / 8;
     id = x * per + min(x, rem) + i;
@@ -462,6 +461,61 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void gemm16_kernel(Gemm16<T> G) {
   }
 }
 
+template <typename T, int BM, int BN, int WR, int WC, int ST, bool KA, bool KB>
+__global__ __launch_bounds__(64 * WR * WC, 2) void gemm16_kernel(Gemm16<T> G) {
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  gemm16_tile<T, BM, BN, WR, WC, ST, KA, KB>(G, blockIdx.x, lds);
+}
+
+// out[c] = the sum of G partial rows in column c; NW waves take every NW-th row of 64 columns from c0 on, sixteen loads in flight, and
+// meet in `red` [NW][64]
+template <int NW, typename T> __device__ __forceinline__ void colsum16(const float* part, int G, int N, T* out, int c0, float* red) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = c0 + lane;
+  float s = 0.f;
+  if (c < N) {
+    int g = wave;
+    for (; g + 15 * NW < G; g += 16 * NW) {
+      float v[16];
+#pragma unroll
+      for (int k = 0; k < 16; ++k) v[k] = part[(long long)(g + k * NW) * N + c];
+#pragma unroll
+      for (int k = 0; k < 16; ++k) s += v[k];
+    }
+    for (; g < G; g += NW) s += part[(long long)g * N + c];
+  }
+  red[wave * 64 + lane] = s;
+  __syncthreads();
+  if (wave == 0 && c < N) {
+    float t = 0.f;
+#pragma unroll
+    for (int k = 0; k < NW; ++k) t += red[k * 64 + lane];
+    out[c] = (T)t;
+  }
+}
+
+// The two products of a backward pass and the bias gradient's last sums in one launch: dz is all they wait for, and none of them fills
+// the chip evenly at ordinary sizes.  The product with the longer contraction first, then the other, the sums last.  Measured against the
+// three launches, bf16, us: 4352 x 768 x 2304 (rows x inputs x outputs) 47 / 60, 4352 x 768 x 768 24 / 35, 600 x 4096 x 1024 19 / 30, 34 x 768 x 768
+// 5.8 / 10.5, 64 x 64 x 64 3.4 / 7.6.
+template <typename T> struct Pair16 {
+  Gemm16<T> dx, dw;                                // layouts 1 and 2
+  int dx_first, n0, n01;                           // workgroups of the first product, of both
+  const float* part; int groups, n;                // partial column sums [groups][n]
+  T* dbias;
+};
+template <typename T, int BM, int BN, int WR, int WC, int ST>
+__global__ __launch_bounds__(64 * WR * WC, 2) void gemm16_pair_kernel(Pair16<T> P) {
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  const int id = blockIdx.x;
+  if (id >= P.n01) colsum16<WR * WC>(P.part, P.groups, P.n, P.dbias, (id - P.n01) * 64, reinterpret_cast<float*>(lds));
+  else {
+    const bool first = id < P.n0;
+    const int mine = first ? id : id - P.n0;
+    if (first == (P.dx_first != 0)) gemm16_tile<T, BM, BN, WR, WC, ST, true, false>(P.dx, mine, lds);
+    else gemm16_tile<T, BM, BN, WR, WC, ST, false, false>(P.dw, mine, lds);
+  }
+}
+
 // the partial results of a split contraction, added in split order, through the same epilogue; four columns per thread
 template <typename T>
 __global__ __launch_bounds__(256) void gemm16_join_kernel(const float* __restrict__ part, int splits, int M, int N, Epi16<T> E) {
@@ -629,32 +683,23 @@ __global__ __launch_bounds__(256) void act_bwd16_kernel(const T* __restrict__ dy
 
 template <typename T>
 __global__ __launch_bounds__(1024) void colsum16_join_kernel(const float* __restrict__ part, int G, int N, T* __restrict__ out) {
-  __shared__ float red[16][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
-  float s = 0.f;
-  if (c < N)
-#pragma unroll 4
-    for (int g = wave; g < G; g += 16) s += part[(long long)g * N + c];
-  red[wave][lane] = s;
-  __syncthreads();
-  if (wave == 0 && c < N) {
-    float t = 0.f;
-#pragma unroll
-    for (int k = 0; k < 16; ++k) t += red[k][lane];
-    out[c] = (T)t;
-  }
+  __shared__ float red[16 * 64];
+  colsum16<16>(part, G, N, out, blockIdx.x * 64, red);
 }
 
 // rows of N 16-bit elements at any stride and alignment -> rows of ldp (a multiple of 8) elements, zeros behind the N-th (bits are moved,
-// whatever they stand for)
-__global__ __launch_bounds__(256) void pad16_kernel(const unsigned short* __restrict__ src, long long lds_, unsigned short* __restrict__ dst,
-                                                    long long ldp, int M, int N) {
-  const int vecs = (int)(ldp / 8);
-  const long long total = (long long)M * vecs;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+// whatever they stand for); one or two of them in a launch (workgroups from `first` on take the second)
+struct Pad16 { const unsigned short* src; long long lds; unsigned short* dst; long long ldp; int M, N; };
+__global__ __launch_bounds__(256) void pad16_kernel(Pad16 A, Pad16 B, unsigned first) {
+  const bool second = blockIdx.x >= first;
+  const Pad16& P = second ? B : A;
+  const unsigned block = second ? blockIdx.x - first : blockIdx.x, blocks = second ? gridDim.x - first : first;
+  const int vecs = (int)(P.ldp / 8), N = P.N;
+  const long long total = (long long)P.M * vecs;
+  for (long long i = (long long)block * 256 + threadIdx.x; i < total; i += (long long)blocks * 256) {
     const long long row = i / vecs;
     const int col = (int)(i - row * vecs) * 8;
-    const unsigned short* p = src + row * lds_ + col;
+    const unsigned short* p = P.src + row * P.lds + col;
     u32x4_t v = {0, 0, 0, 0};
     if (col + 8 <= N) v = ld16(p);
     else {
@@ -662,7 +707,7 @@ __global__ __launch_bounds__(256) void pad16_kernel(const unsigned short* __rest
       for (int e = 0; e < 8; ++e)
         if (col + e < N) v[e >> 1] |= (unsigned)p[e] << (16 * (e & 1));
     }
-    st16(dst + row * ldp + col, v);
+    st16(P.dst + row * P.ldp + col, v);
   }
 }
 
@@ -704,6 +749,46 @@ static Plan16 plan16(int M, int N, int K, int layout) {
   return best;
 }
 
+// The two products of a backward pass in one launch: a form, the splits of each, and the model's time.  The workgroups of the longer
+// steps come first, so a slot takes one after the other: `a` of `na` steps, then `b` of `nb`.
+struct PlanPair16 { int form, dx_first; Plan16 dx, dw; float us; };
+static float pair_steps(long long a, long long na, long long b, long long nb, long long slots) {
+  if (a + b <= slots) return (float)std::max(na, nb);
+  const long long t0 = a / slots * na, busy = a % slots, t1 = busy > 0 ? t0 + na : t0;      // slots - busy are free at t0, busy at t1
+  auto first = [&](long long from) {                                                        // the first end, in steps of nb from `from`, by which b are done
+    long long lo = 0, hi = (t1 - t0) / nb + (b + slots - 1) / slots + 1;
+    while (lo < hi) {
+      const long long mid = (lo + hi) / 2, t = from + mid * nb;
+      const long long done = (t - t0) / nb * (slots - busy) + (t > t1 ? (t - t1) / nb * busy : 0);
+      if (done >= b) hi = mid; else lo = mid + 1;
+    }
+    return from + lo * nb;
+  };
+  return (float)std::max(std::min(first(t0), first(t1)), t1);
+}
+static PlanPair16 plan_pair16(int M, int N, int K) {
+  const int s1 = (N + G16_BK - 1) / G16_BK, s2 = (M + G16_BK - 1) / G16_BK;                 // dX [M][K] over N, dW [N][K] over M
+  PlanPair16 best{-1, 0, {}, {}, 0.f};
+  for (int f = 2; f < 5; ++f) {                    // (products that fill the chip in larger tiles gain nothing from each other)
+    const Form16& F = FORMS16[f];
+    const long long m1 = ((long long)M + F.bm - 1) / F.bm, m2 = ((long long)N + F.bm - 1) / F.bm, n1 = ((long long)K + F.bn - 1) / F.bn;
+    for (int p1 = 1; p1 <= 4 && (p1 == 1 || (m1 * n1 * p1 <= F.slots && s1 / p1 >= 4)); p1 *= 2)
+      for (int p2 = 1; p2 <= 32 && (p2 == 1 || (m2 * n1 * p2 <= F.slots && s2 / p2 >= 4)); p2 += p2 < 4 ? 1 : p2 / 2) {
+        const long long w1 = m1 * n1 * p1, w2 = m2 * n1 * p2, l1 = (s1 + p1 - 1) / p1, l2 = (s2 + p2 - 1) / p2;
+        if ((w1 + w2 + N) * 512 >= 1LL << 32) continue;                                     // (more than a launch counts)
+        const bool first = l1 >= l2;
+        const float n = first ? pair_steps(w1, l1, w2, l2, F.slots) : pair_steps(w2, l2, w1, l1, F.slots);
+        const float more = (float)((w1 + w2 - 1) / F.slots);                                // rounds behind the first: each fills its buffers again
+        float t = F.start + n * (w1 + w2 > 256 ? F.together : F.alone) + F.end * (more + 1.f) + more * (F.slots > 256 ? 2.f : 3.f);
+        if (p1 > 1) t += 4.f + 8.f * (float)p1 * (float)M * (float)K / 12e6f;
+        if (p2 > 1) t += 4.f + 8.f * (float)p2 * (float)N * (float)K / 12e6f;
+        if (best.form < 0 || t < best.us)
+          best = PlanPair16{f, first, {f, (int)m1, (int)n1, p1, t}, {f, (int)m2, (int)n1, p2, t}, t};
+      }
+  }
+  return best;
+}
+
 // Up to 64 rows of x w^T: the few-row form where the model finds it faster (one row of 4096 x 4096: 7.0 us against 8.9 in tiles; 64 rows: 20.4
 // against 12.3; 64 rows of 768 x 768 5.2 against 5.8), and wherever the operands do not lie as tiles need them.
 static bool few16(int M, int N, int K, const Plan16& p) {
@@ -717,6 +802,11 @@ template <typename T, int BM, int BN, int WR, int WC, int ST, bool KA, bool KB> 
   static std::atomic<unsigned long long> told{0};
   allow_lds(reinterpret_cast<const void*>(k), bytes, told);
   hipLaunchKernelGGL(k, dim3((unsigned)(G.tiles_m * G.tiles_n * G.splits)), dim3(64 * WR * WC), bytes, st, G);
+}
+template <typename T> static void gemm16_join(const Gemm16<T>& G, const Plan16& p, const float* ws, hipStream_t st) {
+  if (p.splits < 2) return;
+  const long long work = (long long)G.M * ((G.N + 3) / 4), blocks = (work + 255) / 256;
+  hipLaunchKernelGGL((gemm16_join_kernel<T>), dim3((unsigned)(blocks < 2048 ? blocks : 2048)), dim3(256), 0, st, ws, p.splits, G.M, G.N, G.E);
 }
 template <typename T> static void gemm16_run(Gemm16<T> G, int layout, bool few, const Plan16& p, float* ws, hipStream_t st) {
   if (few) {
@@ -742,10 +832,34 @@ template <typename T> static void gemm16_run(Gemm16<T> G, int layout, bool few, 
   if (layout == 0) go(std::true_type{}, std::true_type{});
   else if (layout == 1) go(std::true_type{}, std::false_type{});
   else go(std::false_type{}, std::false_type{});
-  if (p.splits > 1) {
-    const long long work = (long long)G.M * ((G.N + 3) / 4), blocks = (work + 255) / 256;
-    hipLaunchKernelGGL((gemm16_join_kernel<T>), dim3((unsigned)(blocks < 2048 ? blocks : 2048)), dim3(256), 0, st, ws, p.splits, G.M, G.N, G.E);
-  }
+  gemm16_join(G, p, ws, st);
+}
+
+template <typename T, int BM, int BN, int WR, int WC, int ST> static void pair16_go(const Pair16<T>& P, hipStream_t st) {
+  constexpr int bytes = ST * (BM + BN) * G16_BK * 2;
+  const auto k = gemm16_pair_kernel<T, BM, BN, WR, WC, ST>;
+  static std::atomic<unsigned long long> told{0};
+  allow_lds(reinterpret_cast<const void*>(k), bytes, told);
+  hipLaunchKernelGGL(k, dim3((unsigned)(P.n01 + (P.dbias != nullptr ? (P.n + 63) / 64 : 0))), dim3(64 * WR * WC), bytes, st, P);
+}
+template <typename T> static void pair16_run(Pair16<T> P, const PlanPair16& p, float* ws, hipStream_t st) {
+  float* ws2 = p.dx.splits > 1 ? ws + (size_t)p.dx.splits * P.dx.M * P.dx.N : ws;
+  auto set = [&](Gemm16<T>& G, const Plan16& q, float* part) {
+    G.tiles_m = q.tiles_m;
+    G.tiles_n = q.tiles_n;
+    G.splits = q.splits;
+    G.part = q.splits > 1 ? part : nullptr;
+    return q.tiles_m * q.tiles_n * q.splits;
+  };
+  const int w1 = set(P.dx, p.dx, ws), w2 = set(P.dw, p.dw, ws2);
+  P.dx_first = p.dx_first;
+  P.n0 = p.dx_first ? w1 : w2;
+  P.n01 = w1 + w2;
+  if (p.form == 2) pair16_go<T, 128, 128, 2, 2, 2>(P, st);
+  else if (p.form == 3) pair16_go<T, 128, 128, 2, 2, 4>(P, st);
+  else pair16_go<T, 64, 64, 2, 2, 4>(P, st);
+  gemm16_join(P.dx, p.dx, ws, st);
+  gemm16_join(P.dw, p.dw, ws2, st);
 }
 
 // rows of `cols` elements as tiles are staged from them: 16-byte addresses and ends, and a stride whose 256 rows an offset of 32 bits spans
@@ -815,15 +929,92 @@ extern "C" int hopmi_gemm16(const void* A, long long lda, const void* B, long lo
   return check_launch("hopmi_gemm16");
 }
 
-extern "C" int hopmi_pad16(const void* src, long long lds_, void* dst, long long ldp, int M, int N, void* stream) {
-  if (!src || !dst || M < 1 || N < 1 || lds_ < N || ldp < N || (ldp & 7) || (reinterpret_cast<uintptr_t>(dst) & 15)) {
-    set_error("hopmi_pad16: M=%d N=%d strides %lld -> %lld, or a null or unaligned pointer", M, N, lds_, ldp);
+// What the backward pass launches: the pair, or (form < 0) two products of their own and the bias gradient's sums (3 us of their own
+// beside the products), by the models of both: products in 256 x 256 tiles fill the chip by themselves, and short contractions of many
+// tiles are better off in forms of their own (128 rows of 4096 x 4096: 34 us in three launches, 40 as a pair).
+struct Backward16 { PlanPair16 pair; Plan16 dx, dw; size_t floats; };
+static Backward16 plan_backward16(int M, int N, int K) {
+  Backward16 b;
+  b.dx = plan16(M, K, N, 1);
+  b.dw = plan16(N, K, M, 2);
+  b.pair = plan_pair16(M, N, K);
+  if (b.pair.form >= 0 && b.pair.us > b.dx.us + b.dw.us + 3.f) b.pair.form = -1;
+  const Plan16 &x = b.pair.form >= 0 ? b.pair.dx : b.dx, &w = b.pair.form >= 0 ? b.pair.dw : b.dw;
+  b.floats = (x.splits > 1 ? (size_t)x.splits * M * K : 0) + (w.splits > 1 ? (size_t)w.splits * N * K : 0);
+  return b;
+}
+
+extern "C" size_t hopmi_linear16_bwd_ws_floats(int M, int N, int K) { return g16_sides(M, N, K) ? plan_backward16(M, N, K).floats : 0; }
+
+extern "C" int hopmi_linear16_bwd(const void* dz, long long lddz, const void* w, long long ldw, const void* x, long long ldx, void* dx,
+                                  void* dw, const float* part, void* dbias, int M, int N, int K, int dtype, float* ws, void* stream) {
+  if (!dz || !w || !x || !dx || !dw || (dbias && !part)) { set_error("hopmi_linear16_bwd: null pointer argument"); return HOPMI_EINVAL; }
+  if (!g16_sides(M, N, K) || (dtype != T_BF16 && dtype != T_F16)) {
+    set_error("hopmi_linear16_bwd: M=%d N=%d K=%d (sides of 1 to 2^30) dtype=%d (1 bf16, 2 fp16)", M, N, K, dtype);
     return HOPMI_EINVAL;
   }
-  const long long work = (long long)M * (ldp / 8), blocks = (work + 255) / 256;
-  hipLaunchKernelGGL(pad16_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, static_cast<hipStream_t>(stream),
-                     static_cast<const unsigned short*>(src), lds_, static_cast<unsigned short*>(dst), ldp, M, N);
+  const int n8 = (N + 7) & ~7, k8 = (K + 7) & ~7;
+  if (!g16_direct(dz, lddz, 0) || !g16_direct(w, ldw, 0) || !g16_direct(x, ldx, 0) || lddz < n8 || ldw < k8 || ldx < k8) {
+    set_error("hopmi_linear16_bwd: operands need rows on 16 bytes that end on 16 bytes, with strides up to 2^22 elements (hopmi_pad16)");
+    return HOPMI_EINVAL;
+  }
+  const Backward16 b = plan_backward16(M, N, K);
+  if (b.floats > 0 && !ws) { set_error("hopmi_linear16_bwd: null workspace"); return HOPMI_EINVAL; }
+  if (b.pair.form < 0 && (b.dx.splits == 0 || b.dw.splits == 0)) {
+    set_error("hopmi_linear16_bwd: M=%d N=%d K=%d are more tiles than a launch counts", M, N, K);
+    return HOPMI_EINVAL;
+  }
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  auto go = [&](auto t) {
+    using T = decltype(t);
+    auto product = [&](const void* A, long long lda, const void* B, long long ldb, void* C, int m, int k) {
+      Gemm16<T> G;
+      G.A = static_cast<const T*>(A); G.lda = lda;
+      G.B = static_cast<const T*>(B); G.ldb = ldb;
+      G.M = m; G.N = K; G.K = k;
+      G.E = Epi16<T>{static_cast<T*>(C), K, nullptr, nullptr, 0, nullptr, 0, ACT_NONE};
+      G.part = nullptr; G.tiles_m = G.tiles_n = G.splits = 1;
+      return G;
+    };
+    const Gemm16<T> X = product(dz, lddz, w, ldw, dx, M, N), W = product(dz, lddz, x, ldx, dw, N, M);
+    const int groups = act_bwd_groups(M, N);
+    T* db = static_cast<T*>(dbias);
+    if (b.pair.form >= 0) {
+      pair16_run(Pair16<T>{X, W, 0, 0, 0, part, groups, N, db}, b.pair, ws, st);
+      return;
+    }
+    if (db != nullptr) hipLaunchKernelGGL((colsum16_join_kernel<T>), dim3((N + 63) / 64), dim3(1024), 0, st, part, groups, N, db);
+    gemm16_run(X, 1, false, b.dx, ws, st);
+    gemm16_run(W, 2, false, b.dw, b.dx.splits > 1 ? ws + (size_t)b.dx.splits * M * K : ws, st);
+  };
+  if (dtype == T_BF16) go(__bf16{}); else go(_Float16{});
+  return check_launch("hopmi_linear16_bwd");
+}
+
+static bool pad16_fits(const void* src, long long lds, const void* dst, long long ldp, int M, int N) {
+  if (src && dst && g16_sides(M, N, 1) && lds >= N && ldp >= N && ldp <= 1LL << 31 && !(ldp & 7) && !(reinterpret_cast<uintptr_t>(dst) & 15)) return true;
+  set_error("hopmi_pad16: M=%d N=%d strides %lld -> %lld, or a null or unaligned pointer", M, N, lds, ldp);
+  return false;
+}
+static unsigned pad16_blocks(long long ldp, int M) {
+  const long long blocks = ((long long)M * (ldp / 8) + 255) / 256;
+  return (unsigned)(blocks < 4096 ? blocks : 4096);
+}
+extern "C" int hopmi_pad16(const void* src, long long lds_, void* dst, long long ldp, int M, int N, void* stream) {
+  if (!pad16_fits(src, lds_, dst, ldp, M, N)) return HOPMI_EINVAL;
+  const Pad16 P{static_cast<const unsigned short*>(src), lds_, static_cast<unsigned short*>(dst), ldp, M, N};
+  const unsigned blocks = pad16_blocks(ldp, M);
+  hipLaunchKernelGGL(pad16_kernel, dim3(blocks), dim3(256), 0, static_cast<hipStream_t>(stream), P, P, blocks);
   return check_launch("hopmi_pad16");
+}
+extern "C" int hopmi_pad16_two(const void* src, long long lds_, void* dst, long long ldp, int M, int N, const void* src2, long long lds2,
+                               void* dst2, long long ldp2, int M2, int N2, void* stream) {
+  if (!pad16_fits(src, lds_, dst, ldp, M, N) || !pad16_fits(src2, lds2, dst2, ldp2, M2, N2)) return HOPMI_EINVAL;
+  const Pad16 P{static_cast<const unsigned short*>(src), lds_, static_cast<unsigned short*>(dst), ldp, M, N};
+  const Pad16 Q{static_cast<const unsigned short*>(src2), lds2, static_cast<unsigned short*>(dst2), ldp2, M2, N2};
+  const unsigned first = pad16_blocks(ldp, M), blocks = first + pad16_blocks(ldp2, M2);
+  hipLaunchKernelGGL(pad16_kernel, dim3(blocks), dim3(256), 0, static_cast<hipStream_t>(stream), P, Q, first);
+  return check_launch("hopmi_pad16_two");
 }
 
 extern "C" size_t hopmi_act_bwd16_ws_floats(int M, int N) { return !g16_sides(M, N, 1) ? 0 : (size_t)act_bwd_groups(M, N) * N; }
@@ -835,13 +1026,13 @@ extern "C" int hopmi_act_bwd16(const void* dy, long long ldy, const void* z, lon
     set_error("hopmi_act_bwd16: M=%d N=%d activation=%d dtype=%d, a bad stride, or a null pointer", M, N, act, dtype);
     return HOPMI_EINVAL;
   }
-  if (!dz && !dbias) return HOPMI_OK;
+  if (!dz && !ws) return HOPMI_OK;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int groups = act_bwd_groups(M, N);
   auto go = [&](auto t) {
     using T = decltype(t);
     hipLaunchKernelGGL((act_bwd16_kernel<T>), dim3((N + 511) / 512, groups), dim3(256), 0, st, static_cast<const T*>(dy), ldy,
-                       static_cast<const T*>(z), ldz, static_cast<T*>(dz), ldd, dbias ? ws : nullptr, M, N, act);
+                       static_cast<const T*>(z), ldz, static_cast<T*>(dz), ldd, ws, M, N, act);
     if (dbias)
       hipLaunchKernelGGL((colsum16_join_kernel<T>), dim3((N + 63) / 64), dim3(1024), 0, st, ws, groups, N, static_cast<T*>(dbias));
   };

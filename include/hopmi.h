@@ -574,12 +574,24 @@ int hopmi_gemm16_direct(const void* p, long long ld, int cols);
 int hopmi_gemm16(const void* A, long long lda, const void* B, long long ldb, int layout, void* C, long long ldc, const void* bias,
                  const void* res, long long ldr, void* z, long long ldz, int act, int M, int N, int K, int dtype, float* ws, void* stream);
 int hopmi_pad16(const void* src, long long lds, void* dst, long long ldp, int M, int N, void* stream);
+/* ... two operands in one launch */
+int hopmi_pad16_two(const void* src, long long lds, void* dst, long long ldp, int M, int N, const void* src2, long long lds2, void* dst2,
+                    long long ldp2, int M2, int N2, void* stream);
 /* dz [M][ldd] = dy act'(z), rows padded with zeros to 8 elements (nullable), and dbias [N] = the column sums of the unrounded dz
- * (nullable; ws: hopmi_act_bwd16_ws_floats(M, N) floats, fixed summation order).  z [M][ldz >= N rounded up to 8], rows on 16 bytes;
+ * (nullable; ws: hopmi_act_bwd16_ws_floats(M, N) floats, fixed summation order; ws without dbias: the partial sums are left in it for
+ * hopmi_linear16_bwd).  z [M][ldz >= N rounded up to 8], rows on 16 bytes;
  * act 0 takes no z. */
 size_t hopmi_act_bwd16_ws_floats(int M, int N);
 int hopmi_act_bwd16(const void* dy, long long ldy, const void* z, long long ldz, void* dz, long long ldd, void* dbias, float* ws, int act,
                     int M, int N, int dtype, void* stream);
+
+/* The backward products of y = x w^T, dx [M][K] = dz w and dw [N][K] = dz^T x, and dbias [N] (nullable) from the partial sums that
+ * hopmi_act_bwd16(M, N) left in `part`: one launch where that is faster than three (and the joins of split contractions).  dz [M][lddz],
+ * w [N][ldw], x [M][ldx]: rows on 16 bytes, backed by whole 16-byte vectors, with zeros behind the last element of dz's; strides of up to
+ * 2^22 elements.  ws: hopmi_linear16_bwd_ws_floats(M, N, K) floats.  Bitwise reproducible. */
+size_t hopmi_linear16_bwd_ws_floats(int M, int N, int K);
+int hopmi_linear16_bwd(const void* dz, long long lddz, const void* w, long long ldw, const void* x, long long ldx, void* dx, void* dw,
+                       const float* part, void* dbias, int M, int N, int K, int dtype, float* ws, void* stream);
 
 /* Global gradient norm and clipping: *norm (device, fp32) = the 2-norm over all `count` tensors, c = min(1, max_norm / (*norm + 1e-6)),
  * and outs[t] = c grads[t]: outs NULL scales in place (nothing is written when c = 1), otherwise outs[t] is an fp32 tensor of the same

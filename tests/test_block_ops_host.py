@@ -140,3 +140,24 @@ def test_tangents_and_pending_negations_are_refused():
     for call in (lambda: ops.layer_norm(n), lambda: ops.linear_act(n, w), lambda: ops.linear_act(x, w, n[0])):
         with pytest.raises(_lib.HopmiError, match="negation"):
             call()
+
+
+def test_linear16_bwd_entry_point_refuses():
+    L = _lib.lib()
+
+    def call(dz=ONE, lddz=64, w=ONE, ldw=72, x=ONE, ldx=72, dx=ONE, dw=ONE, part=ONE, db=ONE, M=100, N=64, K=72, dt=1, ws=ONE):
+        return L.hopmi_linear16_bwd(dz, lddz, w, ldw, x, ldx, dx, dw, part, db, M, N, K, dt, ws, None)
+
+    for kw in (dict(dz=None), dict(w=None), dict(x=None), dict(dx=None), dict(dw=None), dict(part=None)):
+        assert call(**kw) == -1 and "null" in _last(), kw
+    for kw in (dict(M=0), dict(N=0), dict(K=0), dict(dt=0), dict(M=(1 << 30) + 1)):
+        assert call(**kw) == -1 and "M=" in _last(), kw
+    odd = ctypes.c_void_p(24)
+    for kw in (dict(dz=odd), dict(w=odd), dict(x=odd), dict(lddz=56), dict(ldw=76), dict(ldx=64), dict(lddz=60, N=60), dict(K=73), dict(ldx=1 << 23)):
+        assert call(**kw) == -1 and "16 bytes" in _last(), kw
+    assert L.hopmi_linear16_bwd_ws_floats(16000, 40, 40) > 0 and L.hopmi_linear16_bwd_ws_floats(65, 40, 72) == 0
+    assert L.hopmi_linear16_bwd_ws_floats(0, 40, 72) == 0
+    assert call(M=16000, N=40, K=40, ws=None) == -1 and "workspace" in _last()
+    two = lambda **kw: L.hopmi_pad16_two(ONE, 5, ONE, kw.get("ldp", 8), 4, 5, ONE, 5, kw.get("dst2", ONE), 8, kw.get("M2", 4), 5, None)
+    assert two(ldp=12) == -1 and two(dst2=ctypes.c_void_p(8)) == -1 and two(M2=0) == -1 and "pad16" in _last()
+    assert call(M=1 << 30, N=1 << 22, K=1 << 22, lddz=1 << 22, ldw=1 << 22, ldx=1 << 22) == -1 and "more tiles" in _last()

@@ -277,6 +277,40 @@ def test_linear_act_large_weight_gradient():
     _check_linear(200, 3600, 4008, torch.float16, "none", True, False, True)
 
 
+# backward products that share a launch: either one first, splits in either contraction, sums of one and of many row groups, ragged sides
+PAIRED = [(4352, 768, 2304), (2171, 1021, 427), (300, 1021, 427), (4000, 72, 3600), (16000, 40, 40), (16000, 768, 72), (65, 72, 1200),
+          (8192, 1024, 1024), (4352, 768, 768), (128, 4096, 4096), (70, 1, 2000), (3000, 2000, 1)]
+
+
+@pytest.mark.parametrize("dtype,act,bias", [("bf16", "gelu", True), ("fp16", "none", True), ("bf16", "silu", False)])
+@pytest.mark.parametrize("M,K,N", PAIRED)
+def test_linear_act_both_products(M, K, N, dtype, act, bias):
+    _check_linear(M, K, N, TYPES[dtype], act, bias, False, True)
+
+
+def test_linear16_bwd_entry_point():
+    """Both products and the bias gradient's sums by one C call, and nothing written next to them."""
+    L, t = _lib.lib(), torch.bfloat16
+    g = _rng(77)
+    st = torch.cuda.current_stream().cuda_stream
+    for M, K, N in ((65, 72, 40), (300, 1024, 432), (34, 768, 768), (2176, 768, 776)):
+        dz, w, x = _randn(g, M, N).to(t), _randn(g, N, K).to(t), _randn(g, M, K).to(t)
+        out = torch.full((M * K + N * K + N + 24,), 7.0, device=_dev(), dtype=t)
+        dx, dw, db = out[8:8 + M * K], out[16 + M * K:16 + M * K + N * K], out[24 + M * K + N * K:]
+        part = torch.empty(L.hopmi_act_bwd16_ws_floats(M, N), device=_dev())
+        ws = torch.empty(max(1, L.hopmi_linear16_bwd_ws_floats(M, N, K)), device=_dev())
+        assert L.hopmi_act_bwd16(dz.data_ptr(), N, None, 0, None, 0, None, part.data_ptr(), 0, M, N, 1, st) == 0
+        assert L.hopmi_linear16_bwd(dz.data_ptr(), N, w.data_ptr(), K, x.data_ptr(), K, dx.data_ptr(), dw.data_ptr(), part.data_ptr(),
+                                    db.data_ptr(), M, N, K, 1, ws.data_ptr(), st) == 0
+        D, W, X = dz.double(), w.double(), x.double()
+        for got, a, b, n in ((dx.view(M, K), D, W, N), (dw.view(N, K), D.t(), X, M)):
+            want = a @ b
+            check(got, want, _half_step(t) * want.abs() + (n + 2) * 2 * U32 * (a.abs() @ b.abs()) + _tiny(t), f"{M}x{K}x{N}")
+        check(db, D.sum(0), _half_step(t) * D.sum(0).abs() + (M + 2) * U32 * D.abs().sum(0) + _tiny(t), "db")
+        gaps = torch.cat([out[:8], out[8 + M * K:16 + M * K], out[16 + M * K + N * K:24 + M * K + N * K]])
+        assert (gaps == 7.0).all()
+
+
 def test_linear_act_operands_as_they_lie():
     """Row strides, offsets that break the alignment, a transposed operand, leading axes, broadcast residuals and gradients."""
     g = _rng(11)
