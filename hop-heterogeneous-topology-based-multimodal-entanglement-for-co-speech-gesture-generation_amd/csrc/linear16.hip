@@ -620,8 +620,9 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void gemm16_few_kernel(Gemm16<T> G)
 
 // dz = dY act'(z) (rows padded with zeros to ldd, a multiple of 8; null: not wanted) and the partial column sums of the UNROUNDED dz of
 // each row group, part [gridDim.y][N] (null: not wanted).  A wave takes 512 columns of every fourth row of its group.  Bound: HBM (two
-// reads, one write): 16384 x 4096 bf16 gelu 83-87 us (4.7 TB/s), 4352 x 2304 16.7 (3.6 TB/s: five rows per wave do not hide the first's
-// latency).
+// reads, one write): 16384 x 4096 bf16 gelu 77 us (5.2 TB/s), 4352 x 2304 14.7 (4.1).  Six workgroups per CU with one row at a time hide the
+// latency best: with two rows in flight per wave (more registers) 80 and 17.4, with four 87 and 18.7; on eight or four workgroups per CU
+// 81 and 14.7, 78 and 16.2.
 template <typename T>
 __global__ __launch_bounds__(256) void act_bwd16_kernel(const T* __restrict__ dy, long long ldy, const T* __restrict__ z, long long ldz,
                                                         T* __restrict__ dz, long long ldd, float* __restrict__ part, int M, int N, int act) {
@@ -639,22 +640,14 @@ __global__ __launch_bounds__(256) void act_bwd16_kernel(const T* __restrict__ dy
     for (int e = 0; e < 8; ++e) s[e] += g[e];
   };
   if (left >= 8) {
-    for (long long row = first; row < M; row += 2 * step) {      // two rows' loads in flight
-      u32x4_t gv[2], zv[2];
+    for (long long row = first; row < M; row += step) {
+      const u32x4_t gv = ld16(dy + row * ldy + col);
+      u32x4_t zv;                                                // (finish() looks at it where there is an activation)
+      if (act != ACT_NONE) zv = ld16(z + row * ldz + col);
+      float g[8];
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
-        if (row + k * step < M) {
-          gv[k] = ld16(dy + (row + k * step) * ldy + col);
-          if (act != ACT_NONE) zv[k] = ld16(z + (row + k * step) * ldz + col);
-        }
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-        if (row + k * step < M) {
-          float g[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) g[e] = vget(gv[k], e, dy);
-          finish(row + k * step, g, zv[k]);
-        }
+      for (int e = 0; e < 8; ++e) g[e] = vget(gv, e, dy);
+      finish(row, g, zv);
     }
   } else if (left > 0) {                                         // the rows' ends (those of z and dz are padded to 8)
     for (long long row = first; row < M; row += step) {
@@ -874,7 +867,7 @@ static bool g16_sides(int M, int N, int K) {
 static int act_bwd_groups(int M, int N) {
   const int strips = (N + 511) / 512;
   const long long quads = ((long long)M + 3) / 4;
-  long long g = 1024 / strips;
+  long long g = 1536 / strips;
   g = g < 1 ? 1 : g;
   return (int)(quads < g ? quads : g);
 }
