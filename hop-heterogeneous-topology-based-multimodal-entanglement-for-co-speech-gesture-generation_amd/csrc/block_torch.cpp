@@ -69,10 +69,12 @@ bool wants_grad(const OptTensor& t) { return has(t) && t->requires_grad(); }
 OptTensor dense(const OptTensor& t) { return has(t) && !t->is_contiguous() ? OptTensor(t->contiguous()) : t; }
 
 // What the kernels would not see: they read memory, and neither a tangent nor a pending negation is in it.
+void plain_values(const char* what, const Tensor& t) {
+  if (t._fw_grad(0).defined()) refuse(what, ": no forward-mode derivative");
+  if (t.is_neg()) refuse(what, ": a tensor with a pending negation (.resolve_neg() makes a plain one)");
+}
 void plain_values(const char* what, const OptTensor& t) {
-  if (!has(t)) return;
-  if (t->_fw_grad(0).defined()) refuse(what, ": no forward-mode derivative");
-  if (t->is_neg()) refuse(what, ": a tensor with a pending negation (.resolve_neg() makes a plain one)");
+  if (has(t)) plain_values(what, *t);
 }
 void on_device(const Tensor& first, const char* what) {
   if (!first.is_cuda()) refuse(what, ": the operand is on ", first.device(), "; this operator only runs on a ROCm device (no CPU fallback)");
@@ -86,6 +88,8 @@ struct Rows {
   Tensor t;
   int64_t ld = 0;
   int m = 0, n = 0;
+  const void* inside = nullptr;                    // rows in a part of t
+  const void* data() const { return inside != nullptr ? inside : t.const_data_ptr(); }
 };
 Rows rows(const Tensor& x, int64_t width) {
   const int64_t m = x.numel() / width;
@@ -177,7 +181,9 @@ Tensor layer_norm(const Tensor& x, const OptTensor& w0, const OptTensor& b0, dou
     refuse("layer_norm: x has shape ", x.sizes(), " and type ", x.scalar_type(), " (fp32, bf16 or fp16 with a last axis of at least 1)");
   if (d > MOST_WIDTH) refuse("layer_norm: x has shape ", x.sizes(), ": a last axis of up to 2^29");
   if (!(eps >= 0.0)) refuse("layer_norm: eps=", eps);
-  for (const OptTensor& t : {OptTensor(x), w0, b0}) plain_values("layer_norm", t);
+  plain_values("layer_norm", x);
+  plain_values("layer_norm", w0);
+  plain_values("layer_norm", b0);
   on_device(x, "layer_norm");
   for (const auto& [name, t] : {std::pair<const char*, const OptTensor&>{"weight", w0}, {"bias", b0}}) {
     if (!has(t)) continue;
@@ -199,7 +205,7 @@ constexpr int FEW_ROWS = 64;                       // up to here layout 0 takes 
 constexpr int64_t MOST = int64_t(1) << 22;         // longest row that the tiled products address
 constexpr int64_t MOST_ROWS = int64_t(1) << 30;
 
-bool direct(const Rows& r) { return L.hopmi_gemm16_direct(r.t.const_data_ptr(), r.ld, r.n) != 0; }
+bool direct(const Rows& r) { return L.hopmi_gemm16_direct(r.data(), r.ld, r.n) != 0; }
 // as hopmi_gemm16 takes it: as it lies where its rows start and end on 16 bytes, else copied into rows padded with zeros
 Rows padding(const Rows& r) {
   const int64_t ld = (int64_t(r.n) + 7) / 8 * 8;
@@ -229,7 +235,7 @@ void gemm(const Rows& a, const Rows& b, int layout, const Tensor& c, int M, int 
   const size_t n = L.hopmi_gemm16_ws_floats(M, N, K, layout);
   Tensor ws;
   if (n > 0) ws = at::empty({(int64_t)n}, c.options().dtype(at::kFloat));
-  check(L.hopmi_gemm16(a.t.const_data_ptr(), a.ld, b.t.const_data_ptr(), b.ld, layout, out(c), N, ptr(bias), ptr(res.t), res.ld, out(z),
+  check(L.hopmi_gemm16(a.data(), a.ld, b.data(), b.ld, layout, out(c), N, ptr(bias), ptr(res.t), res.ld, out(z),
                        z.defined() ? z.size(1) : 0, act, M, N, K, code(c.scalar_type()), fout(ws), stream(c)), "hopmi_gemm16");
 }
 
@@ -260,16 +266,14 @@ struct LinearActFn : torch::autograd::Function<LinearActFn> {
     // (padded copies, where the product needed them, serve the backward's products too)
     const bool px = o.x.m > FEW_ROWS && !direct(rows(x, x.size(-1))), pw = o.x.m > FEW_ROWS && !direct(rows(w, w.size(1)));
     ctx->save_for_backward({x, w, o.z, px ? o.x.t : Tensor(), pw ? o.w.t : Tensor()});
-    ctx->saved_data["act"] = act;
-    ctx->saved_data["bias"] = has(bias);
-    ctx->saved_data["res"] = has(res);
+    ctx->saved_data["call"] = act | (has(bias) ? 4 : 0) | (has(res) ? 8 : 0);
     return o.y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grad) {
     const variable_list s = ctx->get_saved_variables();
     const Tensor &x = s[0], &w = s[1], &z = s[2];
-    const int act = (int)ctx->saved_data["act"].toInt();
-    const bool bias = ctx->saved_data["bias"].toBool(), res = ctx->saved_data["res"].toBool();
+    const int call = (int)ctx->saved_data["call"].toInt(), act = call & 3;
+    const bool bias = call & 4, res = call & 8;
     size_t edge = 0;
     const bool need_x = ctx->needs_input_grad(edge++), need_w = ctx->needs_input_grad(edge++);
     const bool need_b = bias && ctx->needs_input_grad(edge++), need_r = res && ctx->needs_input_grad(edge++);
@@ -286,20 +290,24 @@ struct LinearActFn : torch::autograd::Function<LinearActFn> {
       if (need_w) g[1] = M > 0 ? at::empty({N, K}, w.options()) : at::zeros({N, K}, w.options());
       if (need_b) g[2] = M > 0 ? at::empty({N}, w.options()) : at::zeros({N}, w.options());
       if (M > 0 && (need_x || need_w || need_b)) {
-        const bool plain = act == 0 && direct(d);  // dz is dy as it lies there
-        Rows dz = d;
-        if (!plain && (need_x || need_w)) {
-          dz.ld = (N + 7) / 8 * 8;
-          dz.t = at::empty({M, dz.ld}, x.options());
-        }
-        const bool make = dz.t.unsafeGetTensorImpl() != d.t.unsafeGetTensorImpl();
+        const bool make = (act != 0 || !direct(d)) && (need_x || need_w);       // else dz is dy as it lies there
         const bool both = need_x && need_w;        // (with the bias gradient's last sums in the same launch)
-        Tensor ws;
-        if (make || need_b) {
-          if (need_b) ws = at::empty({(int64_t)L.hopmi_act_bwd16_ws_floats(M, (int)N)}, x.options().dtype(at::kFloat));
-          check(L.hopmi_act_bwd16(d.t.const_data_ptr(), d.ld, ptr(z), z.defined() ? z.size(1) : 0, make ? out(dz.t) : nullptr, dz.ld,
-                                  both ? nullptr : out(g[2]), fout(ws), act, M, (int)N, code(x.scalar_type()), stream(x)), "hopmi_act_bwd16");
+        // one piece of scratch memory: dz, the bias gradient's partial sums, the split contractions' partial results
+        const int64_t ldz = (N + 7) / 8 * 8, z_floats = make ? (M * ldz / 2 + 3) / 4 * 4 : 0;
+        const int64_t part_floats = need_b ? ((int64_t)L.hopmi_act_bwd16_ws_floats(M, (int)N) + 3) / 4 * 4 : 0;
+        const int64_t ws_floats = both ? (int64_t)L.hopmi_linear16_bwd_ws_floats(M, (int)N, (int)K) : 0;
+        Tensor scratch;
+        float* mem = nullptr;
+        if (z_floats + part_floats + ws_floats > 0) {
+          scratch = at::empty({z_floats + part_floats + ws_floats}, x.options().dtype(at::kFloat));
+          mem = fout(scratch);
         }
+        Rows dz = d;
+        if (make) dz = Rows{scratch, ldz, M, (int)N, mem};
+        float *part = need_b ? mem + z_floats : nullptr, *ws = mem + z_floats + part_floats;
+        if (make || need_b)
+          check(L.hopmi_act_bwd16(d.data(), d.ld, ptr(z), z.defined() ? z.size(1) : 0, make ? mem : nullptr, dz.ld, both ? nullptr : out(g[2]),
+                                  part, act, M, (int)N, code(x.scalar_type()), stream(x)), "hopmi_act_bwd16");
         auto kept = [](const Tensor& p, const Tensor& t) {          // (the forward's padded copy, if there is one)
           Rows r = rows(t, t.size(-1));
           if (!p.defined()) return r;
@@ -311,11 +319,8 @@ struct LinearActFn : torch::autograd::Function<LinearActFn> {
         if (both) {
           Rows pw = kept(s[4], w), px = kept(s[3], x);
           operands(pw, px);
-          const size_t n = L.hopmi_linear16_bwd_ws_floats(M, (int)N, (int)K);
-          Tensor ws2;
-          if (n > 0) ws2 = at::empty({(int64_t)n}, x.options().dtype(at::kFloat));
-          check(L.hopmi_linear16_bwd(dz.t.const_data_ptr(), dz.ld, pw.t.const_data_ptr(), pw.ld, px.t.const_data_ptr(), px.ld, out(g[0]), out(g[1]),
-                                     fout(ws), out(g[2]), M, (int)N, (int)K, code(x.scalar_type()), fout(ws2), stream(x)), "hopmi_linear16_bwd");
+          check(L.hopmi_linear16_bwd(dz.data(), dz.ld, pw.data(), pw.ld, px.data(), px.ld, out(g[0]), out(g[1]), part, out(g[2]), M, (int)N,
+                                     (int)K, code(x.scalar_type()), ws_floats > 0 ? ws : nullptr, stream(x)), "hopmi_linear16_bwd");
         } else if (need_x) gemm(dz, operand(kept(s[4], w)), 1, g[0], M, (int)K, (int)N, OptTensor(), Rows{}, Tensor(), 0);
         else if (need_w) gemm(dz, operand(kept(s[3], x)), 2, g[1], (int)N, (int)K, M, OptTensor(), Rows{}, Tensor(), 0);
       }
@@ -328,7 +333,10 @@ struct LinearActFn : torch::autograd::Function<LinearActFn> {
 Tensor linear_act(const Tensor& x0, const Tensor& w0, const OptTensor& b0, const OptTensor& r0, int64_t act) {
   Tensor x = x0, w = w0;
   OptTensor b = b0, r = r0;
-  for (const OptTensor& t : {OptTensor(x), OptTensor(w), b, r}) plain_values("linear_act", t);
+  plain_values("linear_act", x);
+  plain_values("linear_act", w);
+  plain_values("linear_act", b);
+  plain_values("linear_act", r);
   if (at::autocast::is_autocast_enabled(at::kCUDA)) {
     const at::ScalarType t = at::autocast::get_autocast_dtype(at::kCUDA);
     x = x.to(t);
@@ -341,8 +349,12 @@ Tensor linear_act(const Tensor& x0, const Tensor& w0, const OptTensor& b0, const
   same_device(x, "bias", b);
   same_device(x, "residual", r);
   if (code(x.scalar_type()) < 1) refuse("linear_act: x is ", x.scalar_type(), ": bf16 or fp16 (fp32 products: ops.linear)");
-  for (const auto& [name, t] : {std::pair<const char*, OptTensor>{"w", w}, {"bias", b}, {"residual", r}})
-    if (has(t) && t->scalar_type() != x.scalar_type()) refuse("linear_act: `", name, "` is ", t->scalar_type(), ", x ", x.scalar_type(), ": one type for all operands");
+  auto same_type = [&](const char* name, at::ScalarType t) {
+    if (t != x.scalar_type()) refuse("linear_act: `", name, "` is ", t, ", x ", x.scalar_type(), ": one type for all operands");
+  };
+  same_type("w", w.scalar_type());
+  if (has(b)) same_type("bias", b->scalar_type());
+  if (has(r)) same_type("residual", r->scalar_type());
   if (x.dim() < 1 || w.dim() != 2 || w.size(1) != x.size(-1) || w.size(0) < 1 || w.size(1) < 1)
     refuse("linear_act: x ", x.sizes(), " and w ", w.sizes(), " (N, K) do not fit, or have an empty side");
   if (w.size(0) > MOST || w.size(1) > MOST) refuse("linear_act: w ", w.sizes(), ": sides of up to 2^22");
