@@ -23,7 +23,7 @@
 // over the time; the same product of the BLAS library on the same card; a product of 8192^3 runs there at 1590 TFLOP/s):
 //   16384 x 4096 x 4096   x w^T 405 (1357 TFLOP/s; library 365)   dX 408 (1347; 420)   dW 405 (1357; 470)
 //   4352 x 768 -> 2304    x w^T 24.1 (640; 26.8)                   dX 22.9 (672; 25.4)  dW 29.9 (515; 36.3)
-//   one row, 768 -> 2304  3.6 (few-row form: 3.5 MB of W)          34 rows, 768 -> 768 with bias and residual 6.0
+//   one row, 768 -> 2304  3.6 (few-row form: 3.5 MB of W)          34 rows, 768 -> 768 with bias and residual 5.2
 // With bias, gelu, residual and the kept pre-activation (three more streams of the result's size) 16384 x 4096 x 4096 takes 470-490,
 // 4352 x 768 -> 2304 32.
 #include "t16_dev.h"
@@ -782,11 +782,13 @@ static PlanPair16 plan_pair16(int M, int N, int K) {
   return best;
 }
 
-// Up to 64 rows of x w^T: the few-row form where the model finds it faster (one row of 4096 x 4096: 7.0 us against 8.9 in tiles; 64 rows: 20.4
-// against 12.3; 64 rows of 768 x 768 5.2 against 5.8), and wherever the operands do not lie as tiles need them.
+// Up to 64 rows of x w^T: the few-row form where the models find it faster (its own: a start, and per stretch of the contraction W's
+// fragment and each row's), and wherever the operands do not lie as tiles need them.  Measured, few rows / tiles, us: one row of 768 x 768
+// 3.2 / 5.2, of 4096 x 4096 8.7 / 10.8; 34 rows of 768 x 768 4.8 / 5.6, of 2304 -> 768 9.1 / 7.6, of 4096 x 4096 15.7 / 11.8; 64 rows of 128 x 128 3.2 /
+// 3.9, of 768 x 768 5.9 / 5.6; one row of 1024 -> 16384, four workgroups per CU, 9.1 / 8.4.
 static bool few16(int M, int N, int K, const Plan16& p) {
-  const float per_k = M <= 16 ? 1.6e-3f : M <= 32 ? 2.4e-3f : 4.2e-3f;
-  return p.splits == 0 || 3.f + (float)((N + 16 * 512 - 1) / (16 * 512)) * (float)K * per_k <= p.us;
+  const float per_k = 1.05e-3f + 5.2e-5f * (float)M, rounds = (float)((N + 16 * 256 - 1) / (16 * 256));
+  return p.splits == 0 || 2.5f + rounds * (float)K * per_k <= p.us - 0.2f;
 }
 
 template <typename T, int BM, int BN, int WR, int WC, int ST, bool KA, bool KB> static void gemm16_go(const Gemm16<T>& G, hipStream_t st) {
@@ -806,6 +808,7 @@ template <typename T> static void gemm16_run(Gemm16<T> G, int layout, bool few, 
     const dim3 grid((G.N + 15) / 16), block(64 * FEW_WAVES);
     if (G.M <= 16) hipLaunchKernelGGL((gemm16_few_kernel<T, 1>), grid, block, 0, st, G);
     else if (G.M <= 32) hipLaunchKernelGGL((gemm16_few_kernel<T, 2>), grid, block, 0, st, G);
+    else if (G.M <= 48) hipLaunchKernelGGL((gemm16_few_kernel<T, 3>), grid, block, 0, st, G);
     else hipLaunchKernelGGL((gemm16_few_kernel<T, 4>), grid, block, 0, st, G);
     return;
   }
