@@ -539,7 +539,7 @@ class GraphedTrainStep:
 
     def _recording_failed(self, cap, exc):
         """An exception interrupted a recording: `self._stream` is still inside a stream capture.  Measured on this runtime
-        (tools/probes/capture_failure_probe.py, profiles/r04_capture_probe.txt): a capture LEFT OPEN aborts the process at
+        (profiles/r04_capture_probe.txt): a capture LEFT OPEN aborts the process at
         interpreter exit (SIGABRT out of the graph object's destructor); a healthy capture (a Python-level error, and most illegal
         calls, which this runtime refuses without invalidating the capture) ends the ordinary way; an INVALIDATED one (e.g. a
         device-wide synchronize under capture) makes hipStreamEndCapture answer with the invalidation error and the stream keeps
