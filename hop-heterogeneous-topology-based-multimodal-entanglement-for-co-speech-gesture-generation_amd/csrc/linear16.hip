@@ -77,9 +77,10 @@ __device__ __forceinline__ float act_fwd(float z, int act) {
   }
   return top;
 }
-__device__ __forceinline__ float act_grad(float z, int act) {
-  if (act == ACT_NONE) return 1.f;
-  if (act == ACT_RELU) return z > 0.f ? 1.f : 0.f;
+// g act'(z).  relu selects: what arrives at an inactive unit is dropped, an infinity or a NaN too (0 times it would be NaN).
+__device__ __forceinline__ float act_bwd(float g, float z, int act) {
+  if (act == ACT_NONE) return g;
+  if (act == ACT_RELU) return z > 0.f ? g : 0.f;
   float d;                                         // act'(-u); act'(u) = 1 - act'(-u)
   if (act == ACT_GELU) {
     const float u = bounded(z, 14.f), e = __builtin_amdgcn_exp2f(u * u * -0.72134752044448170f);
@@ -89,7 +90,7 @@ __device__ __forceinline__ float act_grad(float z, int act) {
     const float r = __builtin_amdgcn_rcpf(1.f + e), s = e * r;       // the sigmoids of u and of -u
     d = s * fmaf(-u, r, 1.f);
   }
-  return z > 0.f ? 1.f - d : d;
+  return g * (z > 0.f ? 1.f - d : d);
 }
 
 // V (4 or 8) consecutive elements at any element address
@@ -633,7 +634,7 @@ __global__ __launch_bounds__(256) void act_bwd16_kernel(const T* __restrict__ dy
   auto finish = [&](long long row, float (&g)[8], const u32x4_t& zv) {
     if (act != ACT_NONE) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) g[e] *= act_grad(vget(zv, e, dy), act);
+      for (int e = 0; e < 8; ++e) g[e] = act_bwd(g[e], vget(zv, e, dy), act);
     }
     if (dz != nullptr) st16(dz + row * ldd + col, vpack(g, dy));
 #pragma unroll

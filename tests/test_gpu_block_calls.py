@@ -1,0 +1,57 @@
+"""GPU (-m gpu): calls of the trainable block's operators (layer_norm, linear_act, GradClip / clip_grad_norm_) next to the ordinary ones:
+values that are not finite, tensors that stand for their memory in another way, operands that change between the passes."""
+import pytest
+import torch
+
+import hopmi
+
+pytestmark = pytest.mark.gpu
+ops = hopmi.ops
+TYPES = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
+
+
+def _dev():
+    assert torch.cuda.is_available(), "GPU tests need the MI355X"
+    return torch.device("cuda:0")
+
+
+def _rng(seed):
+    return torch.Generator(device=_dev()).manual_seed(seed)
+
+
+def _randn(g, *shape):
+    return torch.randn(*shape, generator=g, device=_dev())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("M,K,N", [(8, 16, 24), (100, 40, 21), (300, 72, 64)])
+def test_relu_drops_what_arrives_at_inactive_units(M, K, N, dtype):
+    """dz = where(z > 0, dy, 0): an infinity or a NaN of dy at an inactive unit changes nothing, at an active one it stays in its row of
+    dx, its row of dw and its bias gradient."""
+    t = TYPES[dtype]
+    g = _rng(M + N)
+    leaves = [v.to(t).requires_grad_() for v in (_randn(g, M, K), _randn(g, N, K), _randn(g, N))]
+    y = ops.linear_act(*leaves, activation="relu")
+    dy = _randn(g, M, N).to(t)
+    off = y.detach() == 0
+    plain = torch.where(off, torch.zeros_like(dy), dy)
+    want = torch.autograd.grad(y, leaves, plain, retain_graph=True)
+    bad = dy.clone()
+    k = off.flatten().nonzero()[:, 0]
+    for i, v in enumerate((float("inf"), float("-inf"), float("nan"))):
+        bad.view(-1)[k[i::3]] = v
+    got = torch.autograd.grad(y, leaves, bad, retain_graph=True)
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+    row, col = (~off).nonzero()[0].tolist()
+    bad[row, col] = float("inf")
+    dx, dw, db = torch.autograd.grad(y, leaves, bad)
+    assert not dx[row].isfinite().any() and not dw[col].isfinite().any() and db[col] == float("inf")
+    rows, cols = torch.arange(M, device=_dev()) != row, torch.arange(N, device=_dev()) != col
+    assert torch.equal(dx[rows], want[0][rows]) and torch.equal(dw[cols], want[1][cols]) and torch.equal(db[cols], want[2][cols])
+    # a NaN before the activation is not above zero either
+    b = leaves[2].detach().clone()
+    b[0] = float("nan")
+    b.requires_grad_()
+    y = ops.linear_act(leaves[0], leaves[1], b, activation="relu")
+    gb = torch.autograd.grad(y, b, dy)[0]
+    assert y[:, 0].isnan().all() and gb[0] == 0
