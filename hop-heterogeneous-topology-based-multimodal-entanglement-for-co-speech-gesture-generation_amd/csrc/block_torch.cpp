@@ -158,7 +158,7 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
     {
       at::NoGradGuard no_grad;
       const Rows r = rows(x, x.size(-1));
-      const Tensor dy = grad[0].contiguous();
+      const Tensor dy = grad[0].resolve_neg().contiguous();   // (autograd may hand over a view with a pending negation)
       if (need_x) g[0] = at::empty(x.sizes(), x.options());
       if (need_w) g[1] = r.m > 0 ? at::empty(w.sizes(), w.options()) : at::zeros(w.sizes(), w.options());
       if (need_b) g[2] = r.m > 0 ? at::empty(b.sizes(), b.options()) : at::zeros(b.sizes(), b.options());
@@ -285,7 +285,7 @@ struct LinearActFn : torch::autograd::Function<LinearActFn> {
       at::NoGradGuard no_grad;
       const int64_t N = w.size(0), K = w.size(1);
       if (need_x) g[0] = at::empty(x.sizes(), x.options());
-      const Rows d = rows(dy, N);
+      const Rows d = rows(dy.resolve_neg(), N);    // (autograd may hand over a view with a pending negation)
       const int M = d.m;
       if (need_w) g[1] = M > 0 ? at::empty({N, K}, w.options()) : at::zeros({N, K}, w.options());
       if (need_b) g[2] = M > 0 ? at::empty({N}, w.options()) : at::zeros({N}, w.options());

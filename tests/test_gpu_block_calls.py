@@ -55,3 +55,30 @@ def test_relu_drops_what_arrives_at_inactive_units(M, K, N, dtype):
     y = ops.linear_act(leaves[0], leaves[1], b, activation="relu")
     gb = torch.autograd.grad(y, b, dy)[0]
     assert y[:, 0].isnan().all() and gb[0] == 0
+
+
+@pytest.mark.parametrize("M,N", [(8, 16), (150, 24), (90, 1), (1, 40)])
+def test_a_gradient_with_a_pending_negation(M, N):
+    """autograd hands a backward pass views whose sign is still to be applied (the imaginary part of a conjugate): dense ones, ones with a
+    single column, strided ones."""
+    g = _rng(M)
+    dy = _randn(g, M, N)
+    wide = _randn(g, M, 2 * N)
+    forms = [(torch._neg_view(-dy), dy), (torch._neg_view(wide[:, :N]), -wide[:, :N]), (torch._neg_view(wide[:, ::2]), -wide[:, ::2]),
+             (torch.complex(dy, dy).conj().imag, -dy)]
+    x, w, b = (_randn(g, *s).requires_grad_() for s in ((M, N), (N,), (N,)))
+    for neg, plain in forms:
+        assert neg.is_neg() and not plain.is_neg()
+        a, c = (torch.autograd.grad(ops.layer_norm(x, w, b), [x, w, b], d) for d in (neg, plain))
+        assert all(torch.equal(p, q) for p, q in zip(a, c))
+    for act in ("none", "gelu"):
+        for need in ((True, True, True), (False, False, True)):
+            leaves = [_randn(g, *s).bfloat16().requires_grad_(n) for s, n in zip(((M, 40), (N, 40), (N,)), need)]
+            wanted = [v for v in leaves if v.requires_grad]
+            for neg, plain in [(torch._neg_view(-dy.bfloat16()), dy.bfloat16()), (torch._neg_view(wide.bfloat16()[:, :N]), -wide.bfloat16()[:, :N])]:
+                a, c = (torch.autograd.grad(ops.linear_act(*leaves, activation=act), wanted, d) for d in (neg, plain))
+                assert all(torch.equal(p, q) for p, q in zip(a, c))
+    # as it comes about: through the imaginary part of a conjugate
+    y = ops.layer_norm(x, w, b)
+    got = torch.autograd.grad((torch.complex(y, 2 * y).conj().imag * dy).sum(), x)[0]
+    assert torch.equal(got, torch.autograd.grad(ops.layer_norm(x, w, b), x, -2 * dy)[0])
