@@ -263,9 +263,7 @@ class GraphedTrainStep:
         self.world = dist.get_world_size(group) if dist.is_available() and dist.is_initialized() else 1
         self.rank = dist.get_rank(group) if self.world > 1 else 0
         self.exchange = self.world > 1 or (force_exchange and dist.is_available() and dist.is_initialized())
-        if self.exchange and getattr(args, "max_grad_norm", None) is not None:
-            raise _lib.HopmiError("hopmi GraphedTrainStep: max_grad_norm needs every rank to hold the whole gradient, and the recorded step shards "
-                                  "the mapping layer's rows over the ranks; steps.train_llm with a GradSync clips")
+        self._refuse_clip()
         self.accel = accelerator if accelerator is not None else _PlainBackward()
         # at least one eager call per phase: besides library handles, every model builds state lazily in its first call
         # (the frozen BERT's operand images, the GRU's packed weights, selection matrices), and some of that cannot be recorded
@@ -289,6 +287,12 @@ class GraphedTrainStep:
         self.sharded = False
         self._pool = None
         self._built = False
+
+    def _refuse_clip(self):
+        # (looked at again in every call: `args` is the caller's and may change after construction)
+        if self.exchange and getattr(self.args, "max_grad_norm", None) is not None:
+            raise _lib.HopmiError("hopmi GraphedTrainStep: max_grad_norm needs every rank to hold the whole gradient, and the recorded step shards "
+                                  "the mapping layer's rows over the ranks; steps.train_llm with a GradSync clips")
 
     # -- one-time device state -------------------------------------------------------------------------------------
     def _build(self, dev):
@@ -604,6 +608,7 @@ class GraphedTrainStep:
         batch = (in_audio, log_melspec, text_token_padded, target_dir_vec, vid_indices)
         if not (self.enabled and in_audio.is_cuda):
             return self._eager(epoch, batch)
+        self._refuse_clip()                          # (before the eager calls too: not in the middle of a run)
         gan = epoch > 10 and self.args.loss_gan_weight > 0.0
         left = self.eager_left.setdefault(gan, self.eager_calls)
         if left > 0:
