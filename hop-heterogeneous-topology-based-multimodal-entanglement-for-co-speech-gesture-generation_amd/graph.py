@@ -614,12 +614,14 @@ class GraphedTrainStep:
         if left > 0:
             self.eager_left[gan] = left - 1
             return self._eager(epoch, batch)
-        key = (gan, torch.is_autocast_enabled(), _steps._MIXED, getattr(self.args, "mixed_precision", None),
-               getattr(self.args, "max_grad_norm", None)) + tuple(
+        key = (gan, torch.is_autocast_enabled(), _steps._MIXED, getattr(self.args, "mixed_precision", None)) + tuple(
             (tuple(t.shape), t.dtype) for t in batch)
+        limit = getattr(self.args, "max_grad_norm", None)
         rec = self.records.get(key)
-        if rec is not None and rec["frozen"] != self._frozen_versions():
-            # a frozen parameter was modified behind the recordings: they replay tensors derived from the old values
+        if rec is not None and (rec["frozen"] != self._frozen_versions() or rec["limit"] != limit):
+            # a frozen parameter was modified behind the recordings: they replay tensors derived from the old values; or the limit
+            # changed, which a recording holds as a kernel argument.  (The last replay's backward may still be running.)
+            torch.cuda.synchronize(in_audio.device)
             self.records.clear()
             self.eager_left.clear()
             self._pool = torch.cuda.graph_pool_handle()          # (the old pool went with its last graph)
@@ -631,6 +633,7 @@ class GraphedTrainStep:
                 self._build(in_audio.device)
             rec = self.records[key] = self._capture(epoch, batch)
             rec["frozen"] = self._frozen_versions()
+            rec["limit"] = limit
         for dst, src in zip(rec["static"], batch):
             if dst.data_ptr() != src.data_ptr():
                 dst.copy_(src, non_blocking=True)

@@ -82,3 +82,34 @@ def test_a_gradient_with_a_pending_negation(M, N):
     y = ops.layer_norm(x, w, b)
     got = torch.autograd.grad((torch.complex(y, 2 * y).conj().imag * dy).sum(), x)[0]
     assert torch.equal(got, torch.autograd.grad(ops.layer_norm(x, w, b), x, -2 * dy)[0])
+
+
+def test_recorded_step_follows_a_changed_limit(monkeypatch):
+    """args.max_grad_norm may change between calls of a recorded step: the call with the new limit clips by it, and the step is recorded
+    again (it does not stay eager)."""
+    from oracle.golden_util import step_args
+    from test_gpu_graph import _deterministic_draws, _pair
+    _deterministic_draws(monkeypatch)
+    m, d, inp = _pair(9, _dev())
+    batch = (inp["in_audio"], inp["log_melspec"], inp["text"], inp["target_dir_vec"], inp["vid_indices"])
+    g = torch.optim.Adam([p for p in m.parameters() if p.requires_grad], lr=1e-4, betas=(0.5, 0.999))
+    o = torch.optim.Adam(d.parameters(), lr=1e-4, betas=(0.5, 0.999))
+    args = step_args(9)
+    run = hopmi.GraphedTrainStep(args, m, d, g, o, eager_calls=1)
+
+    def call():
+        run(0, *batch)
+        torch.cuda.synchronize()
+        return sum(float(p.grad.double().square().sum()) for p in m.parameters() if p.grad is not None) ** 0.5
+
+    free = [call() for _ in range(3)]
+    assert (run.n_eager, run.n_replay) == (1, 2)
+    for limit, eager, replay in ((0.125 * free[-1], 2, 4), (0.25 * free[-1], 3, 6)):
+        args.max_grad_norm = limit
+        # far below the norm of every step here, so the gradients a step leaves behind have it as theirs: 1e-6 in the formula's
+        # denominator, one rounding per value
+        norms = [call() for _ in range(3)]
+        assert all(abs(n - limit) <= 1e-5 * free[-1] for n in norms), (norms, limit)
+        assert (run.n_eager, run.n_replay) == (eager, replay)
+    args.max_grad_norm = None
+    assert all(call() > 0.5 * free[-1] for _ in range(3)) and (run.n_eager, run.n_replay) == (4, 8)
