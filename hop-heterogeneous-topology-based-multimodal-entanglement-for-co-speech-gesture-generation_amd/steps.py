@@ -93,12 +93,18 @@ def _regularisers(args, outputs, z_context, z_mu, z_logvar, out_rand, z_rand):
     return div_reg, kld
 
 
-def _clip(args, optim):
+def _clip(args, optim, accelerator=None):
     """`args.max_grad_norm` (absent or None: no clipping, as the reference trains): the generator's gradients scaled to that global
-    2-norm in front of its optimizer step (ops.clip_grad_norm_; nothing is read back)."""
+    2-norm in front of its optimizer step (ops.clip_grad_norm_; nothing is read back).  An accelerator that scales the loss takes the
+    scale out of the gradients first (`unscale_gradients`), and one that is still accumulating (`sync_gradients` false: its optimizers
+    do not step) is left alone."""
     limit = getattr(args, "max_grad_norm", None)
-    if limit is not None:
-        _ops.clip_grad_norm_([p for g in optim.param_groups for p in g["params"]], limit)
+    if limit is None or not getattr(accelerator, "sync_gradients", True):
+        return
+    unscale = getattr(accelerator, "unscale_gradients", None)
+    if unscale is not None:
+        unscale(optim)
+    _ops.clip_grad_norm_([p for g in optim.param_groups for p in g["params"]], limit)
 
 
 _CAPTURE = None     # a graph._Capture while a training-step graph is being recorded (see graph.GraphedTrainStep)
@@ -291,7 +297,7 @@ def train_llm(args, epoch, in_audio, log_melspec, text_token_padded, target_dir_
                 loss = loss + gen_error * args.loss_gan_weight
         fetch = _LossFetch(args, gan, huber_loss, kld, div_reg, gen_error, dis_error)
         _backward(accelerator, loss, model)
-        _clip(args, model_optim)
+        _clip(args, model_optim, accelerator)
         model_optim.step()
     return fetch.result()
 

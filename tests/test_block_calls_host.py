@@ -27,3 +27,129 @@ def test_recorded_step_over_ranks_refuses_a_limit_that_is_set_later(tmp_path):
         assert run.n_eager == 0 and run.eager_left == {}
     finally:
         dist.destroy_process_group()
+
+
+# ------------------------------------------------------------------------------------------- clipping inside the training steps
+class _Generator(torch.nn.Module):
+    """The generators' call shapes (train_llm's and train_iter_gan's: the poses come out of the last audio-shaped operand)."""
+
+    def __init__(self, poses):
+        super().__init__()
+        self.lin, self.poses = torch.nn.Linear(4, poses), poses
+
+    def forward(self, *operands):
+        out = self.lin(operands[0] if operands[0].shape[-1] == 4 else operands[2])
+        return out, out.mean(1), None, None
+
+
+class _Scores(torch.nn.Module):
+    def __init__(self, poses):
+        super().__init__()
+        self.lin = torch.nn.Linear(poses, 1)
+
+    def forward(self, poses, text=None):
+        return torch.sigmoid(self.lin(poses).mean(1))
+
+    def update_statistics(self, poses):
+        pass
+
+
+class _Optim:
+    """An SGD optimizer that takes the loss's scale out of the gradients, unless that has been done, and writes down what it steps on."""
+
+    def __init__(self, module, name, log, scale=1.0):
+        self.opt, self.name, self.log, self.scale, self.scaled = torch.optim.SGD(module.parameters(), lr=0.1), name, log, scale, True
+        self.param_groups = self.opt.param_groups
+
+    def zero_grad(self):
+        self.opt.zero_grad()
+
+    def unscale(self):
+        for g in self.param_groups:
+            for p in g["params"]:
+                p.grad.div_(self.scale)
+        self.scaled = False
+
+    def step(self):
+        if self.scaled:
+            self.unscale()
+        self.scaled = True
+        self.log.append(("step", self.name, [p.grad.clone() for g in self.param_groups for p in g["params"]]))
+        self.opt.step()
+
+
+def _trace(monkeypatch, log):
+    """The device operator's place is taken by torch's: what is looked at here is what it is given, and when."""
+    from hopmi import steps
+
+    def clip(params, limit):
+        params = list(params)
+        log.append(("clip", params, limit))
+        return torch.nn.utils.clip_grad_norm_(params, limit)
+
+    monkeypatch.setattr(steps._ops, "clip_grad_norm_", clip)
+    monkeypatch.setattr(steps, "FUSED_LOSSES", False)
+
+
+def _args(**more):
+    return types.SimpleNamespace(loss_regression_weight=600.0, loss_gan_weight=5.0, loss_kld_weight=0.0, loss_reg_weight=0.0, z_type="none",
+                                 loss_warmup=0, n_pre_poses=4, **more)
+
+
+def _norm(ts):
+    return float(torch.cat([t.reshape(-1) for t in ts]).norm())
+
+
+def _llm(args, epoch, accelerator, log):
+    torch.manual_seed(3)
+    g, d = _Generator(27), _Scores(27)
+    audio, target = torch.randn(5, 34, 4), torch.randn(5, 34, 27)
+    opts = [_Optim(m, n, log, accelerator.scale) for m, n in ((g, "generator"), (d, "discriminator"))]
+    hopmi.train_llm(args, epoch, audio, None, None, target, None, g, d, *opts, accelerator)
+    return g
+
+
+class _Accel:
+    """An accelerator that scales the loss, as fp16 training does."""
+
+    def __init__(self, scale, log, **more):
+        self.scale, self.log = scale, log
+        self.__dict__.update(more)
+
+    def backward(self, loss):
+        (loss * self.scale).backward()
+        self.log.append(("backward",))
+
+    def unscale_gradients(self, optimizer=None):
+        self.log.append(("unscale", optimizer.name))
+        optimizer.unscale()
+
+
+@pytest.mark.parametrize("epoch", [0, 11])
+def test_train_llm_clips_unscaled_gradients(epoch, monkeypatch):
+    """Under an accelerator that scales the loss, the limit is one on the gradients, not on their scaled form."""
+    log = []
+    _trace(monkeypatch, log)
+    g = _llm(_args(max_grad_norm=0.5), epoch, _Accel(1024.0, log), log)
+    assert [e[0] for e in log][-4:] == ["backward", "unscale", "clip", "step"] and log[-3][1] == "generator" and log[-1][1] == "generator"
+    assert [id(p) for p in log[-2][1]] == [id(p) for p in g.parameters()] and log[-2][2] == 0.5
+    assert [e[0] for e in log].count("clip") == 1 and [e[0] for e in log].count("unscale") == 1
+    stepped = log[-1][2]
+    # 2^10 scales exactly, so these are the bits of the step without a scale; 16 roundings for a norm of 135 values
+    log.clear()
+    _llm(_args(max_grad_norm=0.5), epoch, _Accel(1.0, log), log)
+    assert abs(_norm(stepped) - 0.5) <= 16 * 2.0 ** -24 and all(torch.equal(a, b) for a, b in zip(stepped, log[-1][2]))
+
+
+def test_train_llm_clips_only_with_a_limit_and_in_front_of_a_step(monkeypatch):
+    """Without a limit the gradients are the optimizer's alone; while an accelerator accumulates, its optimizers do not step."""
+    log = []
+    _trace(monkeypatch, log)
+    for args, more in ((_args(), {}), (_args(max_grad_norm=None), {}), (_args(max_grad_norm=0.5), dict(sync_gradients=False))):
+        log.clear()
+        _llm(args, 0, _Accel(1024.0, log, **more), log)
+        assert [e[0] for e in log] == ["backward", "step"]
+    log.clear()
+    accel = types.SimpleNamespace(backward=lambda loss: loss.backward(), scale=1.0)          # .backward(loss) is all that is asked for
+    _llm(_args(max_grad_norm=0.5), 0, accel, log)
+    assert [e[0] for e in log] == ["clip", "step"]
