@@ -153,3 +153,32 @@ def test_train_llm_clips_only_with_a_limit_and_in_front_of_a_step(monkeypatch):
     accel = types.SimpleNamespace(backward=lambda loss: loss.backward(), scale=1.0)          # .backward(loss) is all that is asked for
     _llm(_args(max_grad_norm=0.5), 0, accel, log)
     assert [e[0] for e in log] == ["clip", "step"]
+
+
+@pytest.mark.parametrize("epoch", [0, 1])
+@pytest.mark.parametrize("limit", [None, 0.25, 1e9])
+def test_train_iter_gan_clips_the_generators_gradients_in_front_of_its_step(epoch, limit, monkeypatch):
+    """backward, clip of exactly the generator's parameters, step; in the discriminator's step nothing is clipped."""
+    def run(args):
+        torch.manual_seed(4)
+        g, d = _Generator(27), _Scores(27)
+        audio, poses = torch.randn(5, 34, 4), torch.randn(5, 34, 27)
+        hopmi.train_iter_gan(args, epoch, torch.zeros(5, 3), audio, poses, None, g, d, _Optim(g, "generator", log), _Optim(d, "discriminator", log))
+        return g
+
+    log = []
+    _trace(monkeypatch, log)
+    run(_args())
+    free = log[:]
+    assert [e[:2] for e in free] == [("step", "discriminator")] * epoch + [("step", "generator")] and _norm(free[-1][2]) > 0.5
+    log.clear()
+    g = run(_args(max_grad_norm=limit))
+    assert [e[0] for e in log] == ["step"] * epoch + (["clip"] if limit is not None else []) + ["step"]
+    if limit is not None:
+        assert [id(p) for p in log[-2][1]] == [id(p) for p in g.parameters()] and log[-2][2] == limit
+    if epoch:
+        assert all(torch.equal(a, b) for a, b in zip(log[0][2], free[0][2]))
+    if limit == 0.25:
+        assert abs(_norm(log[-1][2]) - 0.25) <= 16 * 2.0 ** -24                  # (16 roundings; 1e-6 / norm of the formula is below them)
+    else:
+        assert all(torch.equal(a, b) for a, b in zip(log[-1][2], free[-1][2]))
