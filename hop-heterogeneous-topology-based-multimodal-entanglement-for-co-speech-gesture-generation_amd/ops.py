@@ -2429,6 +2429,8 @@ class LayerNorm(torch.nn.LayerNorm):
             raise _lib.HopmiError(f"hopmi: LayerNorm: normalized_shape={tuple(self.normalized_shape)}: one axis, the last")
 
     def forward(self, x):
+        if tuple(x.shape[-1:]) != tuple(self.normalized_shape):      # (without weights the operator takes any width)
+            raise _lib.HopmiError(f"hopmi: LayerNorm: x has shape {tuple(x.shape)}, normalized_shape is {tuple(self.normalized_shape)}")
         return layer_norm(x, self.weight, self.bias, self.eps)
 
 

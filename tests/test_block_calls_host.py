@@ -29,6 +29,17 @@ def test_recorded_step_over_ranks_refuses_a_limit_that_is_set_later(tmp_path):
         dist.destroy_process_group()
 
 
+@pytest.mark.parametrize("affine", [False, True])
+def test_layer_norm_module_refuses_another_width(affine):
+    """Without weights the operator itself cannot tell: it normalises over whatever the last axis is."""
+    m = ops.LayerNorm(8, elementwise_affine=affine)
+    for shape in ((4, 16), (8, 1), ()):
+        with pytest.raises(_lib.HopmiError, match="normalized_shape"):
+            m(torch.zeros(shape))
+    with pytest.raises(_lib.HopmiError, match="no CPU fallback"):
+        m(torch.zeros(4, 8))
+
+
 # ------------------------------------------------------------------------------------------- clipping inside the training steps
 class _Generator(torch.nn.Module):
     """The generators' call shapes (train_llm's and train_iter_gan's: the poses come out of the last audio-shaped operand)."""
