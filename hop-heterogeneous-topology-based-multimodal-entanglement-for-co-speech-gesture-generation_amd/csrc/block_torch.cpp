@@ -412,7 +412,8 @@ struct ClipPlan {
         refuse("GradClip: tensors[", i, "] (", t.scalar_type(), ", shape ", t.sizes(), ") is not an fp32, bf16 or fp16 tensor without gaps "
                "(.contiguous() makes one)");
       if (t.is_neg()) refuse("GradClip: tensors[", i, "] has a pending negation (.resolve_neg() makes a plain tensor)");
-      const void* p = t.const_data_ptr();
+      // (in place the tensor is written: one whose memory is a lazy copy of another's gets its own first)
+      const void* p = into ? t.const_data_ptr() : t.mutable_data_ptr();
       const int c = code(t.scalar_type());
       if (!first && (n[i] != t.numel() || dt[i] != c)) refuse("GradClip: tensors[", i, "] is not the tensor that the plan was made for any more");
       if (p != src[i]) separate = false;

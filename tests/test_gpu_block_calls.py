@@ -113,3 +113,21 @@ def test_recorded_step_follows_a_changed_limit(monkeypatch):
         assert (run.n_eager, run.n_replay) == (eager, replay)
     args.max_grad_norm = None
     assert all(call() > 0.5 * free[-1] for _ in range(3)) and (run.n_eager, run.n_replay) == (4, 8)
+
+
+def test_grad_clip_of_lazy_copies():
+    """A tensor that shares its memory with another until one of them is written: clipping in place writes it, so the other keeps its
+    values; read only (out given), it may go on sharing."""
+    base = torch.full((1000,), 2.0, device=_dev())
+    a, b = torch._lazy_clone(base), torch._lazy_clone(base)
+    plan = ops.GradClip([a, b])
+    norm = plan.clip_(1.0)
+    want = (2000 * 4) ** 0.5
+    assert abs(float(norm) - want) <= 2 * 2.0 ** -24 * want
+    assert (base == 2).all() and all(torch.allclose(t, torch.full_like(t, 2 / want), rtol=1e-6) for t in (a, b))
+    c, o = torch._lazy_clone(base), torch.zeros(1000, device=_dev())
+    ops.GradClip([c], out=[o]).clip_(1.0)
+    assert (base == 2).all() and (c == 2).all() and torch._C._is_cow_tensor(c) and (o < 1).all()
+    d = torch._lazy_clone(base)                                                  # written through a lazy output: only that one
+    ops.GradClip([torch.ones(1000, device=_dev())], out=[d]).clip_(1.0)
+    assert (base == 2).all() and (d < 1).all()
