@@ -102,12 +102,15 @@ Rows rows(const Tensor& x, int64_t width) {
   return r;
 }
 
-// What a backward pass hands out under create_graph: gradients whose own backward pass, to whatever they were made of, is an error.
-variable_list once(variable_list g, const variable_list& made_of) {
+// What a backward pass hands out under create_graph: gradients whose own backward pass, to whatever they were made of, is an error.  They
+// were made of `dy` and of the first `operands` operands of the node that is being run (by its edges, whether it saved them or not).
+variable_list once(variable_list g, const Tensor& dy, size_t operands) {
   if (!at::GradMode::is_enabled()) return g;
   torch::autograd::edge_list edges;
-  for (const Tensor& t : made_of)
-    if (t.defined() && t.requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(t));
+  const auto node = torch::autograd::get_current_node();
+  for (size_t i = 0; i < operands; ++i)
+    if (node->next_edge(i).is_valid()) edges.push_back(node->next_edge(i));
+  if (dy.requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(dy));
   if (edges.empty()) return g;
   auto e = std::make_shared<torch::autograd::Error>("hopmi: this operator is differentiable once: its backward pass has no gradient", std::move(edges));
   for (Tensor& t : g)
@@ -151,7 +154,7 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
     size_t edge = 0;
     const bool need_x = ctx->needs_input_grad(edge++);
     const bool need_w = w.defined() && ctx->needs_input_grad(edge++);
-    const bool need_b = b.defined() && ctx->needs_input_grad(edge++);
+    const bool need_b = b.defined() && ctx->needs_input_grad(edge++);      // (edge: how many operands there are)
     variable_list g(4);
     if (!grad[0].defined()) return g;
     const c10::DeviceGuard guard(x.device());
@@ -171,7 +174,7 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
                                     out(g[1]), out(g[2]), fout(ws), r.m, r.n, dt, stream(x)), "hopmi_layernorm_bwd");
       }
     }
-    return once(std::move(g), {x, w, b, grad[0]});
+    return once(std::move(g), grad[0], edge);
   }
 };
 
@@ -326,7 +329,7 @@ struct LinearActFn : torch::autograd::Function<LinearActFn> {
       }
       if (need_r) g[3] = dy;
     }
-    return once(std::move(g), {x, w, dy});
+    return once(std::move(g), dy, 2 + (bias && act != 0));      // (the bias is in z, and z in act'(z))
   }
 };
 

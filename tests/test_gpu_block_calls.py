@@ -131,3 +131,34 @@ def test_grad_clip_of_lazy_copies():
     d = torch._lazy_clone(base)                                                  # written through a lazy output: only that one
     ops.GradClip([torch.ones(1000, device=_dev())], out=[d]).clip_(1.0)
     assert (base == 2).all() and (d < 1).all()
+
+
+@pytest.mark.parametrize("act", ["none", "relu", "gelu", "silu"])
+def test_a_second_derivative_is_refused_for_every_operand(act):
+    """linear_act's first gradients depend on the bias through act'(z): that way too leads to the error, not to a missing gradient."""
+    g = _rng(4)
+    x, w, b, r = (_randn(g, *s).bfloat16().requires_grad_() for s in ((80, 16), (24, 16), (24,), (80, 24)))
+    gx, gw, gb = torch.autograd.grad(ops.linear_act(x, w, b, r, act).sum(), [x, w, b], create_graph=True)
+    for first in (gx, gw, gb):
+        for leaf in [x, w] + [b] * (act != "none"):
+            with pytest.raises(RuntimeError, match="differentiable once"):
+                torch.autograd.grad(first.float().sum(), leaf, allow_unused=True, retain_graph=True)
+        # neither the residual nor, without an activation, the bias is in them
+        assert torch.autograd.grad(first.float().sum(), [r] + [b] * (act == "none"), allow_unused=True, retain_graph=True)[0] is None
+    # only the bias is trained: its gradient is made of it all the same
+    gb = torch.autograd.grad(ops.linear_act(x.detach(), w.detach(), b, activation="gelu").sum(), b, create_graph=True)[0]
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(gb.float().sum(), b)
+    # the incoming gradient
+    dy = torch.ones(80, 24, device=_dev(), dtype=torch.bfloat16).requires_grad_()
+    gx = torch.autograd.grad(ops.linear_act(x, w, b, r, act), x, dy, create_graph=True)[0]
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(gx.float().sum(), dy)
+    # layer norm: each of its operands
+    lx, lw, lb = (_randn(g, *s).requires_grad_() for s in ((80, 16), (16,), (16,)))
+    for ww, bb in ((lw, lb), (lw, None), (None, lb), (None, None)):
+        leaves = [t for t in (lx, ww, bb) if t is not None]
+        for first in torch.autograd.grad(ops.layer_norm(lx, ww, bb).square().sum(), leaves, create_graph=True):
+            for leaf in leaves:
+                with pytest.raises(RuntimeError, match="differentiable once"):
+                    torch.autograd.grad(first.sum(), leaf, retain_graph=True)
