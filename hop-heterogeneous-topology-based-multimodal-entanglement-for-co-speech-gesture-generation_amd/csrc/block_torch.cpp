@@ -59,6 +59,7 @@ void check(int rc, const char* what) {
 }
 void* stream(const Tensor& t) { return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).stream(); }
 
+at::ScalarType type(int code) { return code == 0 ? at::kFloat : code == 1 ? at::kBFloat16 : at::kHalf; }
 int code(at::ScalarType t) { return t == at::kFloat ? 0 : t == at::kBFloat16 ? 1 : t == at::kHalf ? 2 : -1; }
 const void* ptr(const OptTensor& t) { return t.has_value() && t->defined() ? t->const_data_ptr() : nullptr; }
 void* out(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
@@ -145,33 +146,39 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& w, const OptTensor& b, double eps) {
     Tensor stat;
     Tensor y = ln_forward(x, w, b, eps, &stat);
-    ctx->save_for_backward({x, unwrap(w), unwrap(b), stat});
+    // what the wanted gradients read, and nothing else: x behind dx and dw, w behind dx (an operand may change where it is not read)
+    ctx->save_for_backward({x.requires_grad() || wants_grad(w) ? x : Tensor(), x.requires_grad() ? unwrap(w) : Tensor(), stat});
+    ctx->saved_data["call"] = weight_code(x, w, b) | (has(w) ? 4 : 0) | (has(b) ? 8 : 0);
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grad) {
     const variable_list s = ctx->get_saved_variables();
-    const Tensor &x = s[0], &w = s[1], &b = s[2], &stat = s[3];
+    const Tensor &x = s[0], &w = s[1], &stat = s[2];
+    const int call = (int)ctx->saved_data["call"].toInt(), wt = call & 3;
     size_t edge = 0;
     const bool need_x = ctx->needs_input_grad(edge++);
-    const bool need_w = w.defined() && ctx->needs_input_grad(edge++);
-    const bool need_b = b.defined() && ctx->needs_input_grad(edge++);      // (edge: how many operands there are)
+    const bool need_w = (call & 4) && ctx->needs_input_grad(edge++);
+    const bool need_b = (call & 8) && ctx->needs_input_grad(edge++);      // (edge: how many operands there are)
     variable_list g(4);
     if (!grad[0].defined()) return g;
-    const c10::DeviceGuard guard(x.device());
+    const c10::DeviceGuard guard(grad[0].device());
     {
       at::NoGradGuard no_grad;
-      const Rows r = rows(x, x.size(-1));
       const Tensor dy = grad[0].resolve_neg().contiguous();   // (autograd may hand over a view with a pending negation)
+      const int64_t D = dy.size(-1);
+      // (where only the bias is wanted there is no x: dy is read in its place, and the sums made with it are not asked for)
+      const Rows r = rows(x.defined() ? x : dy, D);
+      const auto weights = stat.options().dtype(type(wt));
       if (need_x) g[0] = at::empty(x.sizes(), x.options());
-      if (need_w) g[1] = r.m > 0 ? at::empty(w.sizes(), w.options()) : at::zeros(w.sizes(), w.options());
-      if (need_b) g[2] = r.m > 0 ? at::empty(b.sizes(), b.options()) : at::zeros(b.sizes(), b.options());
+      if (need_w) g[1] = r.m > 0 ? at::empty({D}, weights) : at::zeros({D}, weights);
+      if (need_b) g[2] = r.m > 0 ? at::empty({D}, weights) : at::zeros({D}, weights);
       if (r.m > 0) {
-        const int dt = code(x.scalar_type());
+        const int dt = code(dy.scalar_type());
         Tensor ws;
         if (need_w || need_b) ws = at::empty({(int64_t)L.hopmi_layernorm_bwd_ws_floats(r.m, r.n, dt)}, stat.options());
         const float* mean = static_cast<const float*>(stat.const_data_ptr());
-        check(L.hopmi_layernorm_bwd(r.t.const_data_ptr(), r.ld, dy.const_data_ptr(), mean, mean + r.m, ptr(w), weight_code(x, w, b), out(g[0]),
-                                    out(g[1]), out(g[2]), fout(ws), r.m, r.n, dt, stream(x)), "hopmi_layernorm_bwd");
+        check(L.hopmi_layernorm_bwd(r.t.const_data_ptr(), r.ld, dy.const_data_ptr(), mean, mean + r.m, w.defined() ? w.const_data_ptr() : nullptr, wt,
+                                    out(g[0]), out(g[1]), out(g[2]), fout(ws), r.m, r.n, dt, stream(dy)), "hopmi_layernorm_bwd");
       }
     }
     return once(std::move(g), grad[0], edge);
@@ -264,12 +271,14 @@ Linear16 linear_forward(const Tensor& x, const Tensor& w, const OptTensor& bias,
 
 struct LinearActFn : torch::autograd::Function<LinearActFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptTensor& bias, const OptTensor& res, int64_t act) {
-    const bool keep = act != 0 && (x.requires_grad() || w.requires_grad() || wants_grad(bias));
+    const bool need_x = x.requires_grad(), need_w = w.requires_grad(), keep = act != 0 && (need_x || need_w || wants_grad(bias));
     Linear16 o = linear_forward(x, w, bias, res, (int)act, keep);
-    // (padded copies, where the product needed them, serve the backward's products too)
+    // dx reads w and dw reads x, no gradient anything else (an operand may change where it is not read); where the product took a padded
+    // copy, that serves the backward's products too
     const bool px = o.x.m > FEW_ROWS && !direct(rows(x, x.size(-1))), pw = o.x.m > FEW_ROWS && !direct(rows(w, w.size(1)));
-    ctx->save_for_backward({x, w, o.z, px ? o.x.t : Tensor(), pw ? o.w.t : Tensor()});
+    ctx->save_for_backward({!need_w ? Tensor() : px ? o.x.t : x, !need_x ? Tensor() : pw ? o.w.t : w, o.z});
     ctx->saved_data["call"] = act | (has(bias) ? 4 : 0) | (has(res) ? 8 : 0);
+    ctx->saved_data["k"] = w.size(1);
     return o.y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grad) {
@@ -283,15 +292,18 @@ struct LinearActFn : torch::autograd::Function<LinearActFn> {
     variable_list g(5);
     const Tensor& dy = grad[0];
     if (!dy.defined()) return g;
-    const c10::DeviceGuard guard(x.device());
+    const c10::DeviceGuard guard(dy.device());
     {
       at::NoGradGuard no_grad;
-      const int64_t N = w.size(0), K = w.size(1);
-      if (need_x) g[0] = at::empty(x.sizes(), x.options());
+      const int64_t N = dy.size(-1), K = ctx->saved_data["k"].toInt();
+      const auto opt = at::TensorOptions().device(dy.device()).dtype(dy.scalar_type());
+      at::DimVector shape(dy.sizes().begin(), dy.sizes().end());
+      shape.back() = K;
+      if (need_x) g[0] = at::empty(shape, opt);
       const Rows d = rows(dy.resolve_neg(), N);    // (autograd may hand over a view with a pending negation)
       const int M = d.m;
-      if (need_w) g[1] = M > 0 ? at::empty({N, K}, w.options()) : at::zeros({N, K}, w.options());
-      if (need_b) g[2] = M > 0 ? at::empty({N}, w.options()) : at::zeros({N}, w.options());
+      if (need_w) g[1] = M > 0 ? at::empty({N, K}, opt) : at::zeros({N, K}, opt);
+      if (need_b) g[2] = M > 0 ? at::empty({N}, opt) : at::zeros({N}, opt);
       if (M > 0 && (need_x || need_w || need_b)) {
         const bool make = (act != 0 || !direct(d)) && (need_x || need_w);       // else dz is dy as it lies there
         const bool both = need_x && need_w;        // (with the bias gradient's last sums in the same launch)
@@ -302,7 +314,7 @@ struct LinearActFn : torch::autograd::Function<LinearActFn> {
         Tensor scratch;
         float* mem = nullptr;
         if (z_floats + part_floats + ws_floats > 0) {
-          scratch = at::empty({z_floats + part_floats + ws_floats}, x.options().dtype(at::kFloat));
+          scratch = at::empty({z_floats + part_floats + ws_floats}, opt.dtype(at::kFloat));
           mem = fout(scratch);
         }
         Rows dz = d;
@@ -310,22 +322,15 @@ struct LinearActFn : torch::autograd::Function<LinearActFn> {
         float *part = need_b ? mem + z_floats : nullptr, *ws = mem + z_floats + part_floats;
         if (make || need_b)
           check(L.hopmi_act_bwd16(d.data(), d.ld, ptr(z), z.defined() ? z.size(1) : 0, make ? mem : nullptr, dz.ld, both ? nullptr : out(g[2]),
-                                  part, act, M, (int)N, code(x.scalar_type()), stream(x)), "hopmi_act_bwd16");
-        auto kept = [](const Tensor& p, const Tensor& t) {          // (the forward's padded copy, if there is one)
-          Rows r = rows(t, t.size(-1));
-          if (!p.defined()) return r;
-          r.t = p;
-          r.ld = p.size(1);
-          r.n = (int)p.size(1);
-          return r;
-        };
+                                  part, act, M, (int)N, code(dy.scalar_type()), stream(dy)), "hopmi_act_bwd16");
+        auto kept = [](const Tensor& t) { return rows(t, t.size(-1)); };        // (a padded copy as rows of its own length)
         if (both) {
-          Rows pw = kept(s[4], w), px = kept(s[3], x);
+          Rows pw = kept(w), px = kept(x);
           operands(pw, px);
           check(L.hopmi_linear16_bwd(dz.data(), dz.ld, pw.data(), pw.ld, px.data(), px.ld, out(g[0]), out(g[1]), part, out(g[2]), M, (int)N,
-                                     (int)K, code(x.scalar_type()), ws_floats > 0 ? ws : nullptr, stream(x)), "hopmi_linear16_bwd");
-        } else if (need_x) gemm(dz, operand(kept(s[4], w)), 1, g[0], M, (int)K, (int)N, OptTensor(), Rows{}, Tensor(), 0);
-        else if (need_w) gemm(dz, operand(kept(s[3], x)), 2, g[1], (int)N, (int)K, M, OptTensor(), Rows{}, Tensor(), 0);
+                                     (int)K, code(dy.scalar_type()), ws_floats > 0 ? ws : nullptr, stream(dy)), "hopmi_linear16_bwd");
+        } else if (need_x) gemm(dz, operand(kept(w)), 1, g[0], M, (int)K, (int)N, OptTensor(), Rows{}, Tensor(), 0);
+        else if (need_w) gemm(dz, operand(kept(x)), 2, g[1], (int)N, (int)K, M, OptTensor(), Rows{}, Tensor(), 0);
       }
       if (need_r) g[3] = dy;
     }

@@ -162,3 +162,61 @@ def test_a_second_derivative_is_refused_for_every_operand(act):
             for leaf in leaves:
                 with pytest.raises(RuntimeError, match="differentiable once"):
                     torch.autograd.grad(first.sum(), leaf, retain_graph=True)
+
+
+@pytest.mark.parametrize("M,K,N", [(40, 64, 48), (150, 64, 48), (150, 61, 45)])
+@pytest.mark.parametrize("act", ["none", "silu"])
+def test_an_operand_may_change_where_no_wanted_gradient_reads_it(M, K, N, act):
+    """dx reads w, dw reads x, db neither; layer norm's dx reads x and weight, dweight x, dbias none.  What is not read is not kept: it may
+    be overwritten between the passes (a frozen layer's input by the next in-place operation), and what is read is still watched."""
+    g = _rng(M + K)
+    t = torch.bfloat16
+    x, w, b = _randn(g, M, K).to(t), (_randn(g, N, K) / 8).to(t), _randn(g, N).to(t)
+    dy = _randn(g, M, N).to(t)
+    reads = {0: {1}, 1: {0}, 2: set()}
+    for i in range(3):
+        leaves = [v.clone().requires_grad_(i == k) for k, v in enumerate((x, w, b))]
+        want = torch.autograd.grad(ops.linear_act(*leaves, activation=act), leaves[i], dy)[0]
+        for j in range(3):
+            leaves = [v.clone().requires_grad_(i == k) for k, v in enumerate((x, w, b))]
+            given = [v * 1 for v in leaves]
+            y = ops.linear_act(*given, activation=act)
+            with torch.no_grad():
+                given[j].add_(1)
+            if j in reads[i] and K % 8 == 0:
+                with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                    torch.autograd.grad(y, leaves[i], dy)
+            else:                                                                # (rows copied for the product are the product's own)
+                if j in reads[i] and M <= 64:
+                    continue
+                assert torch.equal(torch.autograd.grad(y, leaves[i], dy)[0], want), (i, j)
+    x, w, b = (_randn(g, *s) for s in ((M, K), (K,), (K,)))
+    dy = _randn(g, M, K)
+    reads = {0: {0, 1}, 1: {0}, 2: set()}
+    for i in range(3):
+        leaves = [v.clone().requires_grad_(i == k) for k, v in enumerate((x, w, b))]
+        want = torch.autograd.grad(ops.layer_norm(*leaves), leaves[i], dy)[0]
+        for j in range(3):
+            leaves = [v.clone().requires_grad_(i == k) for k, v in enumerate((x, w, b))]
+            given = [v * 1 for v in leaves]
+            y = ops.layer_norm(*given)
+            with torch.no_grad():
+                given[j].add_(1)
+            if j in reads[i]:
+                with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                    torch.autograd.grad(y, leaves[i], dy)
+            else:
+                assert torch.equal(torch.autograd.grad(y, leaves[i], dy)[0], want), (i, j)
+
+
+def test_frozen_weights_do_not_keep_the_input():
+    """With w frozen, x is not held by the tape: its memory is free again when the caller lets go of it."""
+    t = torch.bfloat16
+    w = torch.zeros(64, 4096, device=_dev(), dtype=t)
+    leaf = torch.zeros(4096, 4096, device=_dev(), dtype=t).requires_grad_()
+    x = leaf * 1                                                                 # 32 MiB
+    y = ops.linear_act(x, w)
+    held = torch.cuda.memory_allocated()
+    del x
+    assert held - torch.cuda.memory_allocated() >= 32 << 20
+    assert torch.autograd.grad(y.sum(), leaf)[0].shape == leaf.shape
