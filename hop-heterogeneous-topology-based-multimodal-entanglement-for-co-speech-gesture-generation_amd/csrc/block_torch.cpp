@@ -90,6 +90,7 @@ struct Rows {
   int64_t ld = 0;
   int m = 0, n = 0;
   const void* inside = nullptr;                    // rows in a part of t
+  bool copied = false;                             // t is a copy made here, not the tensor itself
   const void* data() const { return inside != nullptr ? inside : t.const_data_ptr(); }
 };
 Rows rows(const Tensor& x, int64_t width) {
@@ -100,6 +101,7 @@ Rows rows(const Tensor& x, int64_t width) {
   r.t = x.dim() == 2 ? x : x.reshape({m, width});
   if ((width > 1 && r.t.stride(1) != 1) || (m > 1 && r.t.stride(0) < width)) r.t = r.t.contiguous();
   r.ld = m > 1 ? r.t.stride(0) : width;
+  r.copied = !r.t.is_alias_of(x);
   return r;
 }
 
@@ -219,7 +221,7 @@ bool direct(const Rows& r) { return L.hopmi_gemm16_direct(r.data(), r.ld, r.n) !
 // as hopmi_gemm16 takes it: as it lies where its rows start and end on 16 bytes, else copied into rows padded with zeros
 Rows padding(const Rows& r) {
   const int64_t ld = (int64_t(r.n) + 7) / 8 * 8;
-  return Rows{at::empty({r.m, ld}, r.t.options()), ld, r.m, r.n};
+  return Rows{at::empty({r.m, ld}, r.t.options()), ld, r.m, r.n, nullptr, true};
 }
 Rows operand(const Rows& r) {
   if (direct(r)) return r;
@@ -273,10 +275,9 @@ struct LinearActFn : torch::autograd::Function<LinearActFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptTensor& bias, const OptTensor& res, int64_t act) {
     const bool need_x = x.requires_grad(), need_w = w.requires_grad(), keep = act != 0 && (need_x || need_w || wants_grad(bias));
     Linear16 o = linear_forward(x, w, bias, res, (int)act, keep);
-    // dx reads w and dw reads x, no gradient anything else (an operand may change where it is not read); where the product took a padded
-    // copy, that serves the backward's products too
-    const bool px = o.x.m > FEW_ROWS && !direct(rows(x, x.size(-1))), pw = o.x.m > FEW_ROWS && !direct(rows(w, w.size(1)));
-    ctx->save_for_backward({!need_w ? Tensor() : px ? o.x.t : x, !need_x ? Tensor() : pw ? o.w.t : w, o.z});
+    // dx reads w and dw reads x, no gradient anything else (an operand may change where it is not read); where the product took a copy
+    // (dense or padded), that serves the backward's products too
+    ctx->save_for_backward({!need_w ? Tensor() : o.x.copied ? o.x.t : x, !need_x ? Tensor() : o.w.copied ? o.w.t : w, o.z});
     ctx->saved_data["call"] = act | (has(bias) ? 4 : 0) | (has(res) ? 8 : 0);
     ctx->saved_data["k"] = w.size(1);
     return o.y;

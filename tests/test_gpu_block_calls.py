@@ -220,3 +220,27 @@ def test_frozen_weights_do_not_keep_the_input():
     del x
     assert held - torch.cuda.memory_allocated() >= 32 << 20
     assert torch.autograd.grad(y.sum(), leaf)[0].shape == leaf.shape
+
+
+@pytest.mark.parametrize("M", [40, 150])
+def test_operands_are_copied_once(M):
+    """A transposed weight, or rows without a common stride, are made dense once, in the forward pass, and the backward pass takes that
+    copy: allocations counted per call."""
+    def count(f):
+        n = torch.cuda.memory_stats()["allocation.all.allocated"]
+        r = f()
+        return r, torch.cuda.memory_stats()["allocation.all.allocated"] - n
+
+    g = _rng(M)
+    t = torch.bfloat16
+    w = (_randn(g, 64, 48).to(t) / 8).t().requires_grad_()                       # (48, 64), contiguous along its rows' number
+    x = _randn(g, 2, M, 64).to(t)[:, :M // 2].transpose(0, 1).requires_grad_()   # rows of two blocks, interleaved: no common stride
+    wd, xd = w.detach().contiguous().requires_grad_(), x.detach().contiguous().requires_grad_()
+    dy = _randn(g, M // 2, 2, 48).to(t)
+    y0, forward = count(lambda: ops.linear_act(xd, wd))
+    want, backward = count(lambda: torch.autograd.grad(y0, [xd, wd], dy))
+    for xx, ww, copies in ((x, wd, 1), (xd, w, 1), (x, w, 2)):
+        y, n = count(lambda: ops.linear_act(xx, ww))
+        assert n == forward + copies and torch.equal(y, y0)
+        got, n = count(lambda: torch.autograd.grad(y, [xx, ww], dy))
+        assert n == backward and all(torch.equal(p, q) for p, q in zip(got, want))
