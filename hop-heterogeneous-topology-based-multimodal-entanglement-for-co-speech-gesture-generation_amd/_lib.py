@@ -114,6 +114,7 @@ SIGNATURES = {
     "hopmi_layernorm_bwd_ws_floats": (ctypes.c_size_t, [_I, _I, _I]),
     "hopmi_layernorm_bwd": (_I, [_VP, _LL, _VP, _VP, _VP, _VP, _I, _VP, _VP, _VP, _VP, _I, _I, _I, _VP]),
     "hopmi_gemm16_ws_floats": (ctypes.c_size_t, [_I, _I, _I, _I]),
+    "hopmi_gemm16_form": (_I, [_I] * 4 + [ctypes.POINTER(_I)] * 2),
     "hopmi_gemm16_direct": (_I, [_VP, _LL, _I]),
     "hopmi_gemm16": (_I, [_VP, _LL, _VP, _LL, _I, _VP, _LL, _VP, _VP, _LL, _VP, _LL, _I, _I, _I, _I, _I, _VP, _VP]),
     "hopmi_pad16": (_I, [_VP, _LL, _VP, _LL, _I, _I, _VP]),
@@ -121,6 +122,7 @@ SIGNATURES = {
     "hopmi_act_bwd16_ws_floats": (ctypes.c_size_t, [_I, _I]),
     "hopmi_act_bwd16": (_I, [_VP, _LL, _VP, _LL, _VP, _LL, _VP, _VP, _I, _I, _I, _I, _VP]),
     "hopmi_linear16_bwd_ws_floats": (ctypes.c_size_t, [_I, _I, _I]),
+    "hopmi_linear16_bwd_form": (_I, [_I] * 3 + [ctypes.POINTER(_I)] * 5),
     "hopmi_linear16_bwd": (_I, [_VP, _LL, _VP, _LL, _VP, _LL, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _VP, _VP]),
     "hopmi_grad_clip_ws_bytes": (ctypes.c_size_t, []),
     "hopmi_grad_clip": (_I, [_VP, _VP, _VP, _VP, _I, ctypes.c_float, _VP, _VP, _VP]),

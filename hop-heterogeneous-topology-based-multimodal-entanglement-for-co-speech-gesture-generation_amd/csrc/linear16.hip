@@ -887,6 +887,18 @@ extern "C" size_t hopmi_gemm16_ws_floats(int M, int N, int K, int layout) {
   return p.splits > 1 ? (size_t)p.splits * M * N : 0;
 }
 
+extern "C" int hopmi_gemm16_form(int M, int N, int K, int layout, int* form, int* splits) {
+  if (!g16_sides(M, N, K) || layout < 0 || layout > 2 || !form || !splits) {
+    set_error("hopmi_gemm16_form: M=%d N=%d K=%d (sides of 1 to 2^30) layout=%d, or a null pointer", M, N, K, layout);
+    return HOPMI_EINVAL;
+  }
+  const Plan16 p = plan16(M, N, K, layout);
+  const bool few = layout == 0 && M <= FEW_ROWS && few16(M, N, K, p);
+  *form = few || p.splits == 0 ? -1 : p.form;
+  *splits = few ? 1 : p.splits;
+  return HOPMI_OK;
+}
+
 extern "C" int hopmi_gemm16_direct(const void* p, long long ld, int cols) { return g16_direct(p, ld, cols) ? 1 : 0; }
 
 extern "C" int hopmi_gemm16(const void* A, long long lda, const void* B, long long ldb, int layout, void* C, long long ldc, const void* bias,
@@ -942,6 +954,21 @@ static Backward16 plan_backward16(int M, int N, int K) {
 }
 
 extern "C" size_t hopmi_linear16_bwd_ws_floats(int M, int N, int K) { return g16_sides(M, N, K) ? plan_backward16(M, N, K).floats : 0; }
+
+extern "C" int hopmi_linear16_bwd_form(int M, int N, int K, int* pair, int* dx_form, int* dx_splits, int* dw_form, int* dw_splits) {
+  if (!g16_sides(M, N, K) || !pair || !dx_form || !dx_splits || !dw_form || !dw_splits) {
+    set_error("hopmi_linear16_bwd_form: M=%d N=%d K=%d (sides of 1 to 2^30), or a null pointer", M, N, K);
+    return HOPMI_EINVAL;
+  }
+  const Backward16 b = plan_backward16(M, N, K);
+  *pair = b.pair.form >= 0;
+  const Plan16 &x = *pair ? b.pair.dx : b.dx, &w = *pair ? b.pair.dw : b.dw;
+  *dx_form = x.splits == 0 ? -1 : x.form;
+  *dx_splits = x.splits;
+  *dw_form = w.splits == 0 ? -1 : w.form;
+  *dw_splits = w.splits;
+  return HOPMI_OK;
+}
 
 extern "C" int hopmi_linear16_bwd(const void* dz, long long lddz, const void* w, long long ldw, const void* x, long long ldx, void* dx,
                                   void* dw, const float* part, void* dbias, int M, int N, int K, int dtype, float* ws, void* stream) {

@@ -571,6 +571,9 @@ int hopmi_layernorm_bwd(const void* x, long long ldx, const void* dy, const floa
  * split order by a second launch: bitwise reproducible). */
 size_t hopmi_gemm16_ws_floats(int M, int N, int K, int layout);
 int hopmi_gemm16_direct(const void* p, long long ld, int cols);
+/* which form a product of these sides takes (operands on 16 bytes): *form = -1 few rows, else the tile form (0: 256 x 256, 1: 192 x 128,
+ * 2: 128 x 128 in two buffers, 3: in four, 4: 64 x 64), *splits = over how many workgroups its contraction goes */
+int hopmi_gemm16_form(int M, int N, int K, int layout, int* form, int* splits);
 int hopmi_gemm16(const void* A, long long lda, const void* B, long long ldb, int layout, void* C, long long ldc, const void* bias,
                  const void* res, long long ldr, void* z, long long ldz, int act, int M, int N, int K, int dtype, float* ws, void* stream);
 int hopmi_pad16(const void* src, long long lds, void* dst, long long ldp, int M, int N, void* stream);
@@ -590,6 +593,8 @@ int hopmi_act_bwd16(const void* dy, long long ldy, const void* z, long long ldz,
  * w [N][ldw], x [M][ldx]: rows on 16 bytes, backed by whole 16-byte vectors, with zeros behind the last element of dz's; strides of up to
  * 2^22 elements.  ws: hopmi_linear16_bwd_ws_floats(M, N, K) floats.  Bitwise reproducible. */
 size_t hopmi_linear16_bwd_ws_floats(int M, int N, int K);
+/* which forms they take, as hopmi_gemm16_form says it; *pair = 1: both in one launch */
+int hopmi_linear16_bwd_form(int M, int N, int K, int* pair, int* dx_form, int* dx_splits, int* dw_form, int* dw_splits);
 int hopmi_linear16_bwd(const void* dz, long long lddz, const void* w, long long ldw, const void* x, long long ldx, void* dx, void* dw,
                        const float* part, void* dbias, int M, int N, int K, int dtype, float* ws, void* stream);
 

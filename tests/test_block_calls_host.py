@@ -193,3 +193,46 @@ def test_train_iter_gan_clips_the_generators_gradients_in_front_of_its_step(epoc
         assert abs(_norm(log[-1][2]) - 0.25) <= 16 * 2.0 ** -24                  # (16 roundings; 1e-6 / norm of the formula is below them)
     else:
         assert all(torch.equal(a, b) for a, b in zip(log[-1][2], free[-1][2]))
+
+
+# -------------------------------------------------------------------------------------------------- which form a product takes
+def test_every_form_of_a_product_has_a_size_on_the_device():
+    """The lists that the device tests run name all reachable forms, and each size still takes the form that it stands for."""
+    import linear_forms as lf
+    L = _lib.lib()
+    for product, sizes in lf.ALONE.items():
+        assert set(sizes) == {(f, s) for f in range(5) for s in (False, True) if not (product == "dw" and f == 1)}, product
+        for want, size in sizes.items():
+            f, s = lf.form(L, product, size)
+            assert (f, s > 1) == want, (product, size)
+    assert {k[0] for k in lf.PAIRED} == {2, 3, 4} and len(lf.PAIRED) == 11 and len(lf.SEPARATE) == 4
+    for want, size in lf.PAIRED.items():
+        pair, f, s, g, t = lf.backward_form(L, size)
+        assert pair == 1 and f == g and (f, s > 1, t > 1) == want, size
+    for want, size in lf.SEPARATE.items():
+        pair, f, s, g, t = lf.backward_form(L, size)
+        assert pair == 0 and (s > 1, t > 1) == want, size
+        assert (f, s) == lf.form(L, "dx", size) and (g, t) == lf.form(L, "dw", size)
+    for blocks, size in lf.FEW.items():
+        assert lf.form(L, "y", size) == (-1, 1) and (size[0] + 15) // 16 == blocks
+
+
+def test_form_queries_refuse_and_agree_with_the_workspaces():
+    import ctypes
+    import linear_forms as lf
+    L = _lib.lib()
+    i = ctypes.c_int()
+    last = lambda: L.hopmi_last_error().decode()
+    for args in ((0, 1, 1, 0), (1, 0, 1, 0), (1, 1, 0, 0), (1, 1, 1, 3), ((1 << 30) + 1, 1, 1, 0)):
+        assert L.hopmi_gemm16_form(*args, ctypes.byref(i), ctypes.byref(i)) == -1 and "hopmi_gemm16_form" in last()
+    assert L.hopmi_gemm16_form(1, 1, 1, 0, None, ctypes.byref(i)) == -1 and "null" in last()
+    p = [ctypes.byref(i)] * 5
+    assert L.hopmi_linear16_bwd_form(0, 1, 1, *p) == -1 and L.hopmi_linear16_bwd_form(1, 1, 1, None, *p[1:]) == -1 and "null" in last()
+    for product, sizes in lf.ALONE.items():
+        for M, K, N in sizes.values():
+            a, b, c, layout = {"y": (M, N, K, 0), "dx": (M, K, N, 1), "dw": (N, K, M, 2)}[product]
+            s = lf.form(L, product, (M, K, N))[1]
+            assert L.hopmi_gemm16_ws_floats(a, b, c, layout) == (s * a * b if s > 1 else 0)
+    for M, K, N in [*lf.PAIRED.values(), *lf.SEPARATE.values()]:
+        _, _, s, _, t = lf.backward_form(L, (M, K, N))
+        assert L.hopmi_linear16_bwd_ws_floats(M, N, K) == (s * M * K if s > 1 else 0) + (t * N * K if t > 1 else 0)
