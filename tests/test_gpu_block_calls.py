@@ -244,3 +244,59 @@ def test_operands_are_copied_once(M):
         assert n == forward + copies and torch.equal(y, y0)
         got, n = count(lambda: torch.autograd.grad(y, [xx, ww], dy))
         assert n == backward and all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@pytest.mark.parametrize("M,K,N", [(40, 64, 48), (150, 61, 45)])
+def test_saved_tensors_that_travel_and_recomputed_blocks(M, K, N):
+    """What the operators keep may be packed away and come back as another tensor (dense, elsewhere), and a block may be run again
+    in its backward pass."""
+    from torch.utils.checkpoint import checkpoint
+    g = _rng(M)
+    t = torch.bfloat16
+    x = _randn(g, M, 2 * K).to(t)[:, ::2].requires_grad_()
+    w, b = (_randn(g, N, K) / 8).to(t).requires_grad_(), _randn(g, N).to(t).requires_grad_()
+    lw, lb = _randn(g, N).requires_grad_(), _randn(g, N).requires_grad_()
+    dy = _randn(g, M, N).to(t)
+    leaves = [x, w, b, lw, lb]
+    block = lambda *v: ops.layer_norm(ops.linear_act(*v[:3], activation="gelu"), v[3], v[4])
+    want = torch.autograd.grad(block(*leaves), leaves, dy)
+    with torch.autograd.graph.save_on_cpu():
+        y = block(*leaves)
+    assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(y, leaves, dy), want))
+    y = checkpoint(block, *leaves, use_reentrant=False)
+    assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(y, leaves, dy), want))
+
+
+def test_calls_from_several_threads():
+    """Forward and backward passes from several Python threads at once, each on a stream of its own."""
+    import threading
+    g = _rng(8)
+    t = torch.bfloat16
+    sets = []
+    for k in range(3):
+        v = [_randn(g, 150 + k, 72).to(t), (_randn(g, 56, 72) / 8).to(t), _randn(g, 56).to(t), _randn(g, 56), _randn(g, 56), _randn(g, 150 + k, 56).to(t)]
+
+        def run(v=v):
+            leaves = [a.clone().requires_grad_() for a in v[:5]]
+            y = ops.layer_norm(ops.linear_act(*leaves[:3], activation="silu"), *leaves[3:])
+            grads = torch.autograd.grad(y, leaves, v[5])
+            out = [torch.empty(a.shape, device=a.device) for a in grads]
+            return [y.detach(), *grads, ops.GradClip(grads, out=out).clip_(0.5), *out]
+
+        sets.append((run, run()))
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(run, want):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got = [run() for _ in range(10)]
+            torch.cuda.current_stream().synchronize()
+        if not all(torch.equal(p, q) for r in got for p, q in zip(r, want)):
+            bad.append(run)
+
+    threads = [threading.Thread(target=work, args=s) for s in sets]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not bad
