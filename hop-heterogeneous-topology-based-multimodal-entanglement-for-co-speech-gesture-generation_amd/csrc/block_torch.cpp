@@ -346,6 +346,8 @@ Tensor linear_act(const Tensor& x0, const Tensor& w0, const OptTensor& b0, const
   plain_values("linear_act", w);
   plain_values("linear_act", b);
   plain_values("linear_act", r);
+  // One type for all: the product's operands are 16-bit ones and its result is one of them (a residual in fp32 would be rounded with the
+  // sum at the latest).  Cast in every call: a copy kept by the weight's identity would be stale after an in-place update.
   if (at::autocast::is_autocast_enabled(at::kCUDA)) {
     const at::ScalarType t = at::autocast::get_autocast_dtype(at::kCUDA);
     x = x.to(t);

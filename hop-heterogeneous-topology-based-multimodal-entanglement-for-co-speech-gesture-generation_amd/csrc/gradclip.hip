@@ -13,6 +13,7 @@
 // Measured (a large copy moves 5.2 TB/s): 65.8 M fp32 values in 172 tensors, nothing to scale: norm 38 us (6.9 TB/s, part of it from the
 // 256 MB cache), the second launch 4; 160 M bf16 values into fp32: norm 87 us (320 MB, while the write-back of the last call's 640 MB of
 // results is still under way; 3.7 TB/s), scale 178 us (960 MB: 5.4 TB/s); 1.1 M fp32 values in 40 tensors: 4.4 + 2.5 us, two launches.
+// In place above the limit (both launches and the host's list): 65.8 M fp32 128 us, 790 MB, bf16 60-65, 1.1 M fp32 12.
 #include "t16_dev.h"
 
 namespace hopmi {

@@ -2438,11 +2438,11 @@ def linear_act(x, w, bias=None, residual=None, activation="none"):
     """activation(x w^T + bias) + residual in one launch (hopmi_gemm16), with gradients for all four operands.
 
     x (..., K), w (N, K), bias (N,) or None, residual broadcastable to (..., N) or None: all bf16 or all fp16 (under autocast all are cast
-    to its type first; fp32 products are `linear`'s).  activation: "none", "relu", "gelu" (erf) or "silu".  Accumulation, bias,
+    to its type first, in every call, the residual too; fp32 products are `linear`'s).  activation: "none", "relu", "gelu" (erf) or "silu".  Accumulation, bias,
     activation and residual are fp32, with one rounding at the end.  Any sizes >= 1 (N and K up to 2^22), strides and alignments; few rows
     take a form that reads w once.  For the backward pass the values before the activation are kept in the operands' type, and dz = dy act'(z) is
-    rounded to it once, in front of the two products; the bias gradient sums the unrounded dz.  No atomics: the same bits every time.
-    Differentiable once."""
+    rounded to it once, in front of the two products; the bias gradient sums the unrounded dz.  Beside them x is kept for w's gradient
+    and w for x's, no operand that no wanted gradient reads.  No atomics: the same bits every time.  Differentiable once."""
     act = _ACT.get(activation)
     if act is None:
         raise _lib.HopmiError(f"hopmi: linear_act: activation={activation!r} (one of {', '.join(_ACT)})")
