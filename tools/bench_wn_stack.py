@@ -30,7 +30,8 @@ SO = os.path.join(ROOT, "tools", "probes", "libhopmi_stamps_stack.so")
 
 def build_stamps():
     src = [os.path.join(PKG, "csrc", f) for f in ("api.hip", "gcn.hip", "wavenet.hip", "wavenet_bwd.hip", "wavenet_stack.hip")]
-    subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared", "-DHOPMI_STAMPS", *(["-DSTK_EXP_XLAT"] if os.environ.get("STK_EXP_XLAT") else []),
+    subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared", "-DHOPMI_STAMPS",
+                    "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
                     "-I" + os.path.join(ROOT, "include"), *src, "-o", SO], check=True)
 
 

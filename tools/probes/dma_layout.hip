@@ -1,6 +1,6 @@
 // Probe: L2 -> LDS staging rate of the fp16 GEMM's operand tiles by LDS-DMA, for the row-major image layout (a tile row = 64 bytes
 // out of a K*2-byte row: half a 128-byte line per request) against a tile-blocked layout (the tile's 8 KiB contiguous).
-//   hipcc --offload-arch=gfx950 -O3 -o dma_layout dma_layout.hip && ./dma_layout
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -o dma_layout dma_layout.hip && ./dma_layout
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <vector>

@@ -12,6 +12,7 @@ SO = os.path.join(ROOT, "tools", "probes", "libhopmi_stamps.so")
 def build():
     src = [os.path.join(PKG, "csrc", f) for f in ("api.hip", "gcn.hip")]
     subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared", "-DHOPMI_STAMPS",
+                    "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
                     "-I" + os.path.join(ROOT, "include"), *src, "-o", SO], check=True)
 
 def main():

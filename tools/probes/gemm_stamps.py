@@ -11,7 +11,8 @@ SO = os.path.join(ROOT, "tools", "probes", "libhopmi_stamps_gemm.so")
 
 def build():
     src = [os.path.join(PKG, "csrc", f) for f in ("api.hip", "gemm.hip")]
-    subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared", "-DHOPMI_STAMPS", "-DHOPMI_GEMM_NO_SCHED",
+    subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared", "-DHOPMI_STAMPS",
+                    "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-DHOPMI_GEMM_NO_SCHED",
                     "-I" + os.path.join(ROOT, "include"), *src, "-o", SO], check=True)
 
 def main():

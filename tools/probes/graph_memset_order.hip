@@ -1,6 +1,6 @@
 // Probe: is a hipMemsetAsync recorded as a graph memset node ordered before the kernel node that follows it in the captured
 // stream, when eager launches are queued on the same stream between replays?  Each replay: memset(sem, 0) -> check kernel
-// (counts words that are not 0, then dirties them).  Build: hipcc --offload-arch=gfx950 -O2 graph_memset_order.hip -o graph_memset_order
+// (counts words that are not 0, then dirties them).  Build: hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O2 graph_memset_order.hip -o graph_memset_order
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdlib>
