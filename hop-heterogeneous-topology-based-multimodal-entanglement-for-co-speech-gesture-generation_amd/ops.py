@@ -2421,7 +2421,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
 
 
 class LayerNorm(torch.nn.LayerNorm):
-    """torch.nn.LayerNorm over the last axis on `layer_norm`: the same parameters and state_dict keys."""
+    """torch.nn.LayerNorm over the last axis on `layer_norm`: the same parameters and state_dict keys.  The output has the input's type,
+    under autocast too (torch's is fp32 there)."""
 
     def __init__(self, *args, **kwargs):
         super().__init__(*args, **kwargs)
