@@ -124,6 +124,8 @@ SIGNATURES = {
     "hopmi_linear16_bwd_ws_floats": (ctypes.c_size_t, [_I, _I, _I]),
     "hopmi_linear16_bwd_form": (_I, [_I] * 3 + [ctypes.POINTER(_I)] * 5),
     "hopmi_linear16_bwd": (_I, [_VP, _LL, _VP, _LL, _VP, _LL, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _VP, _VP]),
+    "hopmi_axis_sum_ws_floats": (ctypes.c_size_t, [_LL] * 3),
+    "hopmi_axis_sum": (_I, [_VP, _I, _VP, _I, _LL, _LL, _LL, _VP, _VP]),
     "hopmi_grad_clip_ws_bytes": (ctypes.c_size_t, []),
     "hopmi_grad_clip": (_I, [_VP, _VP, _VP, _VP, _I, ctypes.c_float, _VP, _VP, _VP]),
     "hopmi_adam_chunk": (_I, []),

@@ -36,7 +36,8 @@ PyObject* g_error = nullptr;                       // _lib.HopmiError
 #define HOPMI_API(X)                                                                                                       \
   X(hopmi_last_error) X(hopmi_layernorm_fwd) X(hopmi_layernorm_bwd_ws_floats) X(hopmi_layernorm_bwd) X(hopmi_gemm16_ws_floats) \
   X(hopmi_gemm16) X(hopmi_gemm16_direct) X(hopmi_pad16) X(hopmi_pad16_two) X(hopmi_act_bwd16_ws_floats) X(hopmi_act_bwd16) \
-  X(hopmi_linear16_bwd_ws_floats) X(hopmi_linear16_bwd) X(hopmi_grad_clip_ws_bytes) X(hopmi_grad_clip)
+  X(hopmi_linear16_bwd_ws_floats) X(hopmi_linear16_bwd) X(hopmi_axis_sum_ws_floats) X(hopmi_axis_sum) X(hopmi_grad_clip_ws_bytes) \
+  X(hopmi_grad_clip)
 struct Api {
 #define X(f) decltype(&::f) f = nullptr;
   HOPMI_API(X)
@@ -251,6 +252,45 @@ void gemm(const Rows& a, const Rows& b, int layout, const Tensor& c, int M, int 
                        z.defined() ? z.size(1) : 0, act, M, N, K, code(c.scalar_type()), fout(ws), stream(c)), "hopmi_gemm16");
 }
 
+// The gradient of an operand of shape `to` that was broadcast to dy's: its sums over the axes along which it was repeated, one run of
+// neighbouring axes after the other, from the last on, in fp32 between them.
+Tensor summed_to(const Tensor& grad, at::IntArrayRef to) {
+  if (grad.numel() == 0) return at::zeros(to, grad.options());
+  Tensor cur = grad.contiguous();
+  struct Run { int64_t size; bool summed; };
+  std::vector<Run> runs;
+  const int64_t lead = cur.dim() - (int64_t)to.size();
+  for (int64_t i = 0; i < cur.dim(); ++i) {
+    const int64_t size = cur.size(i);
+    if (size == 1) continue;
+    const bool summed = i < lead || to[i - lead] == 1;
+    if (!runs.empty() && runs.back().summed == summed) runs.back().size *= size;
+    else runs.push_back({size, summed});
+  }
+  int left = 0;
+  for (const Run& r : runs) left += r.summed;
+  if (left == 0) return cur.view(to);                        // (axes of one element only)
+  int64_t inner = 1;
+  for (size_t k = runs.size(); k-- > 0;) {
+    if (!runs[k].summed) {
+      inner *= runs[k].size;
+      continue;
+    }
+    int64_t outer = 1;
+    for (size_t j = 0; j < k; ++j) outer *= runs[j].size;
+    const bool last = --left == 0;
+    const auto f32 = cur.options().dtype(at::kFloat);
+    const Tensor sums = last ? at::empty(to, grad.options()) : at::empty({outer * inner}, f32);
+    const size_t n = L.hopmi_axis_sum_ws_floats(outer, runs[k].size, inner);
+    Tensor ws;
+    if (n > 0) ws = at::empty({(int64_t)n}, f32);
+    check(L.hopmi_axis_sum(cur.const_data_ptr(), code(cur.scalar_type()), out(sums), code(sums.scalar_type()), outer, runs[k].size, inner, fout(ws),
+                           stream(cur)), "hopmi_axis_sum");
+    cur = sums;
+  }
+  return cur;
+}
+
 struct Linear16 {
   Tensor y, z;
   Rows x, w;                                       // as the product took them
@@ -263,7 +303,7 @@ Linear16 linear_forward(const Tensor& x, const Tensor& w, const OptTensor& bias,
   o.y = at::empty(shape, x.options());
   if (keep) o.z = at::empty({M, (int64_t(N) + 7) / 8 * 8}, x.options());
   if (M == 0) return o;
-  const Rows r = has(res) ? rows(*res, N) : Rows{};
+  const Rows r = has(res) ? rows(res->sizes() == o.y.sizes() ? *res : res->expand(o.y.sizes()), N) : Rows{};
   if (M > FEW_ROWS) {
     operands(o.x, o.w);
   }
@@ -280,6 +320,7 @@ struct LinearActFn : torch::autograd::Function<LinearActFn> {
     ctx->save_for_backward({!need_w ? Tensor() : o.x.copied ? o.x.t : x, !need_x ? Tensor() : o.w.copied ? o.w.t : w, o.z});
     ctx->saved_data["call"] = act | (has(bias) ? 4 : 0) | (has(res) ? 8 : 0);
     ctx->saved_data["k"] = w.size(1);
+    if (wants_grad(res) && res->sizes() != o.y.sizes()) ctx->saved_data["residual"] = res->sizes().vec();
     return o.y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grad) {
@@ -333,7 +374,9 @@ struct LinearActFn : torch::autograd::Function<LinearActFn> {
         } else if (need_x) gemm(dz, operand(kept(w)), 1, g[0], M, (int)K, (int)N, OptTensor(), Rows{}, Tensor(), 0);
         else if (need_w) gemm(dz, operand(kept(x)), 2, g[1], (int)N, (int)K, M, OptTensor(), Rows{}, Tensor(), 0);
       }
-      if (need_r) g[3] = dy;
+      // (a broadcast residual's by kernels of this library's own: see csrc/axis_sum.hip for why)
+      const auto shape_r = ctx->saved_data.find("residual");
+      if (need_r) g[3] = shape_r == ctx->saved_data.end() ? dy : summed_to(dy.resolve_neg(), shape_r->second.toIntVector());
     }
     return once(std::move(g), dy, 2 + (bias && act != 0));      // (the bias is in z, and z in act'(z))
   }
@@ -378,7 +421,6 @@ Tensor linear_act(const Tensor& x0, const Tensor& w0, const OptTensor& b0, const
       bool fits = r->dim() <= (int64_t)shape.size();
       for (int64_t i = 1; fits && i <= r->dim(); ++i) fits = r->size(-i) == 1 || r->size(-i) == shape[shape.size() - i];
       if (!fits) refuse("linear_act: residual of shape ", r->sizes(), " does not broadcast to ", at::IntArrayRef(shape));
-      r = r->expand(shape);
     }
   }
   const c10::DeviceGuard guard(x.device());

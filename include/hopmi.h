@@ -598,6 +598,12 @@ int hopmi_linear16_bwd_form(int M, int N, int K, int* pair, int* dx_form, int* d
 int hopmi_linear16_bwd(const void* dz, long long lddz, const void* w, long long ldw, const void* x, long long ldx, void* dx, void* dw,
                        const float* part, void* dbias, int M, int N, int K, int dtype, float* ws, void* stream);
 
+/* out [outer][inner] = the sums of in [outer][R][inner] (both dense) over its middle axis, in fp32 and a fixed order, one rounding: the gradient
+ * of an operand that was broadcast along it.  dtypes as above (in and out: fp32 or one 16-bit type); up to 2^40 elements.
+ * ws: hopmi_axis_sum_ws_floats(outer, R, inner) floats. */
+size_t hopmi_axis_sum_ws_floats(long long outer, long long R, long long inner);
+int hopmi_axis_sum(const void* in, int in_dtype, void* out, int out_dtype, long long outer, long long R, long long inner, float* ws, void* stream);
+
 /* Global gradient norm and clipping: *norm (device, fp32) = the 2-norm over all `count` tensors, c = min(1, max_norm / (*norm + 1e-6)),
  * and outs[t] = c grads[t]: outs NULL scales in place (nothing is written when c = 1), otherwise outs[t] is an fp32 tensor of the same
  * numel.  grads / outs / numels / dtypes are HOST arrays, read before the call returns (the list travels in the kernels' arguments);

@@ -236,3 +236,24 @@ def test_form_queries_refuse_and_agree_with_the_workspaces():
     for M, K, N in [*lf.PAIRED.values(), *lf.SEPARATE.values()]:
         _, _, s, _, t = lf.backward_form(L, (M, K, N))
         assert L.hopmi_linear16_bwd_ws_floats(M, N, K) == (s * M * K if s > 1 else 0) + (t * N * K if t > 1 else 0)
+
+
+def test_axis_sum_entry_point_refuses():
+    import ctypes
+    L = _lib.lib()
+    one = ctypes.c_void_p(16)                                # (never dereferenced: the checks come first)
+    last = lambda: L.hopmi_last_error().decode()
+    call = lambda a=one, b=one, it=1, ot=1, outer=1, R=100000, inner=768, ws=one: L.hopmi_axis_sum(a, it, b, ot, outer, R, inner, ws, None)
+    assert call(a=None) == -1 and "null" in last()
+    assert call(b=None) == -1 and "null" in last()
+    for kw in (dict(outer=0), dict(R=0), dict(inner=0), dict(outer=-1), dict(R=1 << 41), dict(outer=1 << 30, R=1 << 30), dict(outer=1 << 20, R=1 << 20, inner=2)):
+        assert call(**kw) == -1 and "2^40" in last(), kw
+        assert L.hopmi_axis_sum_ws_floats(kw.get("outer", 1), kw.get("R", 5), kw.get("inner", 768)) == 0
+    for kw in (dict(it=3), dict(ot=-1), dict(it=1, ot=2)):
+        assert call(**kw) == -1 and "dtype" in last(), kw
+    assert L.hopmi_axis_sum_ws_floats(1, 100000, 768) > 0 and call(ws=None) == -1 and "workspace" in last()
+    assert L.hopmi_axis_sum_ws_floats(1000, 100, 768) == 0 and L.hopmi_axis_sum_ws_floats(1, 1, 1) == 0
+    # groups of whole rows: a workspace of at most 1024 partial rows per outer index, never more than the input
+    for outer, R, inner in ((1, 5, 64), (1, 33, 64), (1, 1 << 30, 1), (7, 4097, 3), (1, 2, 1 << 20), (1 << 20, 1 << 10, 1), (3, 1 << 20, 65)):
+        n = L.hopmi_axis_sum_ws_floats(outer, R, inner)
+        assert n % (outer * inner) == 0 and n <= 1024 * outer * inner and n <= outer * R * inner

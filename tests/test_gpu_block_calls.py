@@ -300,3 +300,88 @@ def test_calls_from_several_threads():
     for th in threads:
         th.join()
     assert not bad
+
+
+@pytest.mark.parametrize("M,N,shape", [(16384, 64, (64,)), (4352, 768, (768,)), (4352, 768, (4352, 1)), (4352, 768, (1,)), (64, 16384, (64, 1))])
+def test_a_broadcast_residual_in_a_recorded_backward(M, N, shape):
+    """The residual's gradient is then a sum by torch, which may record more than kernels: every replay against the eager result, with eager
+    work between them."""
+    g = _rng(M + N)
+    t = torch.bfloat16
+    x, w, r = _randn(g, M, 64).to(t), (_randn(g, N, 64) / 8).to(t), _randn(g, *shape).to(t).requires_grad_()
+    dy = _randn(g, M, N).to(t)
+    f = lambda: torch.autograd.grad(ops.linear_act(x, w, None, r), r, dy)[0]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        f()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        out = f()
+    for _ in range(6):
+        dy.copy_(_randn(g, M, N))
+        want = f().clone()
+        (_randn(g, 1000, 1000) @ _randn(g, 1000, 1000)).sum().item()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
+# (shape of x w^T, shape of the residual): each pattern of repeated axes, few and many of them, columns above and below a wave's width
+BROADCAST = [((150, 48), (48,)), ((150, 48), (1, 48)), ((150, 48), (150, 1)), ((150, 48), (1,)), ((150, 48), (1, 1)), ((4352, 768), (768,)),
+             ((4352, 768), (4352, 1)), ((4352, 768), (1,)), ((9, 17, 70), (17, 70)), ((9, 17, 70), (9, 1, 70)), ((9, 17, 70), (9, 17, 1)),
+             ((9, 17, 70), (1, 17, 1)), ((9, 17, 70), (9, 1, 1)), ((3, 5, 7, 33), (5, 1, 33)), ((3, 5, 7, 33), (3, 1, 7, 1)),
+             ((200, 1, 24), (24,)), ((1, 40), (40,)), ((20001, 3), (3,)), ((20001, 3), (20001, 1)), ((2, 3000, 130), (2, 1, 130)),
+             ((70000, 8), (70000, 1)), ((2100, 63), (63,)), ((2100, 64), (64,)), ((2100, 65), (65,)), ((0, 8), (8,)), ((5, 0, 8), (5, 1, 8)),
+             ((1025, 1000), (1,))]
+
+
+@pytest.mark.parametrize("t", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("shape,rshape", BROADCAST)
+def test_gradient_of_a_broadcast_residual(shape, rshape, t):
+    g = _rng(sum(shape) + len(rshape))
+    K = 16
+    x, w = _randn(g, *shape[:-1], K).to(t), (_randn(g, shape[-1], K) / 4).to(t)
+    r = _randn(g, *rshape).to(t).requires_grad_()
+    dy = (_randn(g, *shape) + 0.1).to(t)
+    y = ops.linear_act(x, w, None, r, "gelu")
+    assert torch.equal(y, ops.linear_act(x, w, None, r.detach().expand(shape).contiguous(), "gelu"))
+    wide = torch.full((*shape[:-1], shape[-1] + 5), 7.0, device=_dev(), dtype=t)
+    wide[..., 2:2 + shape[-1]] = dy
+    want = dy.double().sum_to_size(rshape)
+    mags = dy.double().abs().sum_to_size(rshape)
+    n = dy.numel() // max(1, r.numel())
+    for d in (dy, wide[..., 2:2 + shape[-1]]):
+        got = torch.autograd.grad(y, r, d, retain_graph=True)[0]
+        assert got.dtype == t and got.shape == r.shape
+        if n == 0:
+            assert not got.any()
+            continue
+        # half a step of the type, and at most one rounding of 2^-24 of the magnitudes per addition
+        tol = torch.finfo(t).eps / 2 * want.abs() + n * 2.0 ** -24 * mags + torch.finfo(t).tiny * torch.finfo(t).eps
+        # (a sum that rounds past the type's largest value is an infinity: 4352 x 768 values of mean 0.1 add to 334 000, fp16 ends at 65 520)
+        over = want.abs() >= torch.finfo(t).max * (1 + torch.finfo(t).eps / 4)
+        assert (got.double()[over] == want.sign()[over] * float("inf")).all()
+        assert ((got.double() - want).abs() <= tol)[~over].all(), float(((got.double() - want).abs() - tol)[~over].max())
+        assert torch.equal(got, torch.autograd.grad(y, r, d, retain_graph=True)[0])          # the same bits every time
+
+
+def test_axis_sum_writes_nothing_else():
+    """Sums next to other values, of a large and a small axis in both forms, and of a long one that is cut into groups."""
+    from hopmi import _lib
+    L = _lib.lib()
+    st = torch.cuda.current_stream().cuda_stream
+    g = _rng(77)
+    for outer, R, inner in ((1, 4352, 768), (3, 70, 65), (1, 100003, 1), (5, 9, 63), (4099, 12, 3), (1, 1, 1), (2, 50000, 64), (70000, 2, 7),
+                            (70000, 8, 8), (2100, 9, 8), (2100, 5000, 1), (2100, 130, 33), (30, 1, 50), (300000, 3, 2)):
+        for it, ot in ((0, 0), (1, 0), (1, 1), (0, 2)):
+            v = _randn(g, outer, R, inner).to({0: torch.float32, 1: torch.bfloat16}[it])
+            to = {0: torch.float32, 1: torch.bfloat16, 2: torch.float16}[ot]
+            buf = torch.full((outer * inner + 16,), 7.0, device=_dev(), dtype=to)
+            n = L.hopmi_axis_sum_ws_floats(outer, R, inner)
+            ws = torch.full((n + 8,), 5.0, device=_dev())
+            assert L.hopmi_axis_sum(v.data_ptr(), it, buf[8:].data_ptr(), ot, outer, R, inner, ws.data_ptr() if n else None, st) == 0
+            got, want = buf[8:-8].double().view(outer, inner), v.double().sum(1)
+            tol = torch.finfo(to).eps / 2 * want.abs() + R * 2.0 ** -24 * v.double().abs().sum(1)
+            assert ((got - want).abs() <= tol).all() and (buf[:8] == 7).all() and (buf[-8:] == 7).all() and (ws[n:] == 5).all()
